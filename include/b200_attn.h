@@ -201,6 +201,87 @@ int b200_unpack_decode_metadata(const void* packed, int32_t batch, int32_t table
                                 int32_t buffer_table_cols, int64_t* input_ids, int64_t* positions,
                                 int32_t* slot_mapping, int32_t* context_lens, int32_t* block_tables, void* stream);
 
+/* ---- steps with drafted tokens (speculative decoding) -------------------------------------------------------
+ * No counterpart in the reference, which decodes one token per sequence and step.  A step in which every sequence brings
+ * the nodes of a drafted tree: tables for it (b200_step_tables), its attention in every layer (b200_tree_attn, behind
+ * b200_store_kvcache or b200_qk_norm_rope_store with the step's slots), the walk along the sampled tokens
+ * (b200_accept_tree), the accepted nodes' cache rows to their places (b200_compact_kvcache), and what the sequences no
+ * longer need back into the free list (b200_release_blocks).  Lengths and blocks need not come back to the host.
+ *
+ * A tree: node 0 is its root (the last token that was committed), parents[j] < j is the index of node j's parent within
+ * the tree, anything else (-1, say) means that it has none.  Nodes lie in the cache one behind the other, from the cached
+ * length on, whatever their depth. */
+
+/* A step's tables from request lengths.  Requests own rows of `tables` (max_requests, table_cols; row stride table_stride)
+ * and the first owned[r] ids of their row; free_blocks[0 .. pool[0]) is a stack of free ids.  Sequence i of the batch is
+ * request rows[i] (NULL: i) with cached_lens[i] tokens in the cache and new_lens[i] in this step, whose token rows lie one
+ * behind the other (num_tokens in all).  It takes ceil((cached + new) / block_size) - owned blocks (none below zero) from
+ * the stack, which go into its row and owned; the sequences take theirs in the order of the batch.  Written:
+ *   cu_seqlens_q, cu_seqlens_k (buffer_rows + 1), context_lens (buffer_rows): cumulative new and context lengths, and
+ *                 cached + new; rows from `batch` on repeat the totals and have length 0
+ *   slot_mapping, positions (num_tokens): cache slot and position of each token, -1 and 0 behind the last
+ *   block_tables  (batch, table_cols): ids, -1 behind the last
+ *   tree_masks    (num_tokens, mask_words), with `parents` (num_tokens) only: bit n of a node's mask says that it sees node
+ *                 n, an ancestor or itself; its position is then the cached length plus its depth
+ * A sequence is left out (context length 0, slots -1, positions and masks 0, nothing taken) if its row is outside
+ * [0, max_requests) or stands in the batch before, if it needs more than table_cols blocks, has more than 64 * mask_words
+ * nodes, if its tokens do not all fit into num_tokens, or if there are not enough free blocks when its turn comes (then
+ * later ones get none either).  pool[1] is set to the number of sequences left out.  Negative lengths count as 0.
+ * batch is at most 4096, mask_words at most 4.  Outputs must not overlap the inputs.  The launch lets nothing start early. */
+int b200_step_tables(const int32_t* rows, const int32_t* cached_lens, const int32_t* new_lens, const int32_t* parents,
+                     int32_t batch, int32_t num_tokens, int32_t block_size, int32_t* tables, int64_t table_stride,
+                     int32_t table_cols, int32_t max_requests, int32_t* owned, int32_t* free_blocks, int32_t* pool,
+                     int64_t num_blocks, int32_t buffer_rows, int32_t* cu_seqlens_q, int32_t* cu_seqlens_k,
+                     int32_t* context_lens, int32_t* slot_mapping, int64_t* positions, int32_t* block_tables,
+                     uint64_t* tree_masks, int32_t mask_words, void* stream);
+
+/* Request rows[i] (NULL: i) keeps the blocks of its first keep_lens[i] tokens; the others go back onto the stack (their
+ * columns become -1), in the order that undoes b200_step_tables.  A row that stands in the batch before, or outside
+ * [0, max_requests), gives nothing back.  free_blocks has room for num_blocks ids; more are dropped.  Blocks that other
+ * rows use as well must not be given back: keep them, and take them out of `owned`. */
+int b200_release_blocks(const int32_t* rows, const int32_t* keep_lens, int32_t batch, int32_t block_size, int32_t* tables,
+                        int64_t table_stride, int32_t table_cols, int32_t max_requests, int32_t* owned,
+                        int32_t* free_blocks, int32_t* pool, int64_t num_blocks, void* stream);
+
+/* Bytes of workspace that b200_tree_attn needs with this head geometry on the current device, whatever the batch.  It need
+ * not be initialised and holds nothing between calls; calls that may overlap on the GPU need one each. */
+int64_t b200_tree_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim);
+
+/* Attention of a step's nodes over the paged cache, which has their keys and values already.  Sequence i's nodes are query
+ * rows cu_seqlens_q[i] .. cu_seqlens_q[i+1] of q (total_q, num_heads, 128); node j lies at cache position context_lens[i] - T
+ * + j, T their number.  Each sees all positions in front of the nodes, and of these node n where bit n of its row of
+ * tree_masks (total_q, mask_words) is set; with tree_masks NULL those before it and itself (a drafted chain).  Bits of nodes
+ * that the sequence does not have mean nothing; nodes from 64 * mask_words on are seen by none.  A row that sees nothing
+ * (context_lens[i] <= 0 among them) gives zeros.  GQA, scale and numerics as b200_decode_attn; out (total_q, num_heads, 128)
+ * contiguous; rows outside cu_seqlens_q are left as they are.  Keys and values of a sequence's positions must be finite, seen or
+ * not.  At most 128 query heads per kv head, mask_words at most 4.  The same inputs give the same bits on every call. */
+int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache, int64_t num_blocks,
+                   int32_t block_size, const int32_t* block_tables, int64_t bt_row_stride, int32_t bt_cols,
+                   const int32_t* cu_seqlens_q, const int32_t* context_lens, const uint64_t* tree_masks, int32_t mask_words,
+                   void* out, void* workspace, int64_t workspace_bytes, int32_t batch, int32_t total_q, int32_t num_heads,
+                   int32_t num_kv_heads, int32_t head_dim, float scale, void* stream);
+
+/* The walk through each tree: from the root to the child (the first, if there are several) whose draft token equals the
+ * target token of the node it hangs on, and on from there, at most max_path nodes.  target_tokens[r] is what the target
+ * model's sampler gave behind node r, so what comes out are its own samples.  Written per sequence: accepted (nodes on the
+ * path), path (batch, max_path: their indices), tokens (batch, max_path: their target tokens, the step's result), both -1
+ * behind the last, and new_cached_lens = cached_lens + accepted (may be the same array).  Sequences without nodes or with
+ * context_lens[i] <= 0 (left out of the step) accept none. */
+int b200_accept_tree(const int64_t* draft_tokens, const int64_t* target_tokens, const int32_t* parents,
+                     const int32_t* cu_seqlens_q, const int32_t* cached_lens, const int32_t* context_lens, int32_t batch,
+                     int32_t num_tokens, int32_t max_path, int32_t* accepted, int32_t* path, int64_t* tokens,
+                     int32_t* new_cached_lens, void* stream);
+
+/* The accepted nodes' rows to their places, in all planes of a cache (K and V of every layer; plane_stride_bytes apart,
+ * each num_blocks * block_size rows of row_bytes): the row of position start_lens[i] + path[i][k] goes to start_lens[i] + k
+ * for k < accepted[i], path (batch, path_cols) contiguous.  path ascends; entries below their place (path[i][k] < k) are not
+ * moved, nor is anything from or to a position without a block of the cache.  Pure byte copy.  Sequences must not share
+ * the blocks behind their start lengths.  batch is at most 65535. */
+int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_stride_bytes, int64_t row_bytes, int64_t num_blocks,
+                         int32_t block_size, const int32_t* path, int32_t path_cols, const int32_t* accepted,
+                         const int32_t* start_lens, const int32_t* block_tables, int64_t bt_row_stride, int32_t bt_cols,
+                         int32_t batch, void* stream);
+
 /* ---- behind the path: the all-reduce after the output projection, for decode-sized messages ---------------
  * Replaces `dist.all_reduce(y)` in RowParallelLinear.forward (nanovllm/layers/linear.py:149-153) when y is at
  * most b200_small_allreduce_max_bytes() (512 KiB) of bf16: a one-shot sum over plain peer loads and stores.

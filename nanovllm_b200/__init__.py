@@ -9,6 +9,6 @@ and `nanovllm_b200.integration.install()` swaps the layer into an importable nan
 The kernels live in libb200attn.so (C ABI: include/b200_attn.h), built by nanovllm_b200.build.
 """
 from .layers.attention import (Attention, decode_attention, prefill_attention,  # noqa: F401
-                               store_kvcache)
+                               store_kvcache, tree_attention)
 
-__all__ = ["Attention", "store_kvcache", "decode_attention", "prefill_attention"]
+__all__ = ["Attention", "store_kvcache", "decode_attention", "prefill_attention", "tree_attention"]

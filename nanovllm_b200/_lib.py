@@ -43,6 +43,19 @@ SIGNATURES = {
                                           c_int32, c_int32, c_void_p]),
     "b200_unpack_decode_metadata": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                               c_void_p, c_void_p, c_void_p]),
+    "b200_step_tables": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int32,
+                                   c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_int32, c_void_p]),
+    "b200_release_blocks": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p,
+                                      c_void_p, c_int64, c_void_p]),
+    "b200_tree_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32]),
+    "b200_tree_attn": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32, c_void_p,
+                                 c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                 c_int32, c_float, c_void_p]),
+    "b200_accept_tree": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p]),
+    "b200_compact_kvcache": (c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+                                       c_void_p, c_int64, c_int32, c_int32, c_void_p]),
     "b200_small_allreduce_buffer_bytes": (c_int64, []),
     "b200_small_allreduce_state_bytes": (c_int64, []),
     "b200_small_allreduce_max_bytes": (c_int64, []),

@@ -52,6 +52,8 @@ int read_status_decode();
 int read_status_decode_cluster();
 int read_status_prefill_mma();
 int read_status_prefill_tc2();
+int read_status_tree();
+int reset_state_tree();
 int reset_state_decode();
 int reset_state_decode_cluster();
 int reset_state_prefill_mma();

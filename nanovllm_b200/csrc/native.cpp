@@ -12,6 +12,7 @@
 #include <ATen/core/CachingHostAllocator.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -570,6 +571,249 @@ PyObject* py_unpack(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- steps with drafted tokens (engine/block_tables.py, engine/tree_decode.py, layers/attention.py) ---------------
+// All of these take tensors of one device, which need not be the current one: the launch goes to that device's current stream.
+bool same_device(const Tensor& first, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t && t->device() != first.device()) {
+      PyErr_SetString(PyExc_AssertionError, "all tensors must be on one device");
+      return false;
+    }
+  return true;
+}
+bool is_ints(const Tensor* t, at::ScalarType type = at::kInt) { return t->scalar_type() == type && t->is_contiguous(); }
+int32_t* ints(const Tensor* t) { return t ? static_cast<int32_t*>(t->data_ptr()) : nullptr; }
+int64_t* longs(const Tensor* t) { return t ? static_cast<int64_t*>(t->data_ptr()) : nullptr; }
+bool optional_tensor(PyObject* o, const char* what, const Tensor** t) {
+  *t = nullptr;
+  return o == Py_None || (*t = tensor_of(o, what));
+}
+constexpr int64_t kMost = 0x7fffffff;
+
+// The allocator's state: tables (requests, columns), owned (requests), free_blocks (blocks), pool (2).
+bool check_block_state(const Tensor& tables, const Tensor& owned, const Tensor& free_blocks, const Tensor& pool) {
+  const char* bad = nullptr;
+  if (tables.scalar_type() != at::kInt || tables.dim() != 2 || (tables.size(1) > 1 && tables.stride(1) != 1) || tables.size(0) > kMost ||
+      tables.size(1) > kMost || (tables.size(0) > 1 && tables.stride(0) < tables.size(1)))
+    bad = "tables must be int32 (requests, columns) with contiguous rows";
+  else if (!is_ints(&owned) || owned.dim() != 1 || owned.size(0) != tables.size(0))
+    bad = "owned must be int32, one per request";
+  else if (!is_ints(&free_blocks) || free_blocks.dim() != 1)
+    bad = "free_blocks must be int32, one place per block of the cache";
+  else if (!is_ints(&pool) || pool.numel() != 2)
+    bad = "pool must be two int32";
+  if (bad) PyErr_SetString(PyExc_AssertionError, bad);
+  return !bad;
+}
+int64_t table_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1); }
+
+// step_tables(tables, owned, free_blocks, pool, block_size, rows, cached_lens, new_lens, num_tokens, parents, mask_words, out) ->
+// (cu_seqlens_q, cu_seqlens_k, context_lens, slot_mapping, positions, block_tables, tree_masks); rows, parents and out (such a
+// tuple, to be written again) may be None.
+PyObject* py_step_tables(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(12, "step_tables");
+  const Tensor *t[4], *rows, *cached, *fresh, *parents;
+  static const char* names[4] = {"tables", "owned", "free_blocks", "pool"};
+  for (int i = 0; i < 4; ++i)
+    if (!(t[i] = tensor_of(a[i], names[i]))) return nullptr;
+  int block_size, num_tokens, words;
+  if (!as_int(a[4], &block_size) || !optional_tensor(a[5], "rows", &rows) || !(cached = tensor_of(a[6], "cached_lens")) ||
+      !(fresh = tensor_of(a[7], "new_lens")) || !as_int(a[8], &num_tokens) || !optional_tensor(a[9], "parents", &parents) ||
+      !as_int(a[10], &words))
+    return nullptr;
+  if (!all_cuda({t[0], t[1], t[2], t[3], rows, cached, fresh, parents}) ||
+      !same_device(*t[0], {t[1], t[2], t[3], rows, cached, fresh, parents}) || !check_block_state(*t[0], *t[1], *t[2], *t[3]))
+    return nullptr;
+  const int64_t b = cached->numel(), cols = t[0]->size(1);
+  REQUIRE(is_ints(cached) && cached->dim() == 1 && is_ints(fresh) && fresh->dim() == 1 && fresh->numel() == b, "cached_lens and new_lens must be int32, one per sequence");
+  REQUIRE(b <= kMost && (rows ? is_ints(rows) && rows->dim() == 1 && rows->numel() == b : b <= t[0]->size(0)), "rows must be int32, one per sequence");
+  REQUIRE(num_tokens >= 0 && (!parents || (is_ints(parents) && parents->numel() == num_tokens)), "parents must be int32, one per token");
+  REQUIRE(words >= 0 && words <= 4 && (parents != nullptr) == (words > 0), "mask_words must be 1 to 4 with parents, 0 without");
+  const c10::cuda::CUDAGuard guard(t[0]->device());
+  Tensor o[7];
+  int64_t buffer_rows = b;
+  if (a[11] == Py_None) {
+    const auto dev = t[0]->device();
+    const auto make = [&](at::IntArrayRef sizes, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, dev, std::nullopt); };
+    o[0] = make({b + 1}, at::kInt);
+    o[1] = make({b + 1}, at::kInt);
+    o[2] = make({b}, at::kInt);
+    o[3] = make({num_tokens}, at::kInt);
+    o[4] = make({num_tokens}, at::kLong);
+    o[5] = make({b, cols}, at::kInt);
+    if (parents) o[6] = make({num_tokens, words}, at::kLong);
+  } else {
+    Ref outs(PySequence_Fast(a[11], "out must be a sequence of tensors"));
+    if (!outs.o) return nullptr;
+    REQUIRE(PySequence_Fast_GET_SIZE(outs.o) == 7, "out must have seven tensors");
+    static const char* out_names[7] = {"cu_seqlens_q", "cu_seqlens_k", "context_lens", "slot_mapping", "positions", "block_tables", "tree_masks"};
+    for (int i = 0; i < 7; ++i) {
+      PyObject* item = PySequence_Fast_GET_ITEM(outs.o, i);
+      if (i == 6 && !parents) break;
+      const Tensor* x = tensor_of(item, out_names[i]);
+      if (!x || !all_cuda({x}) || !same_device(*t[0], {x})) return nullptr;
+      o[i] = *x;
+    }
+    buffer_rows = o[2].numel();
+    REQUIRE(is_ints(&o[0]) && is_ints(&o[1]) && is_ints(&o[2]) && is_ints(&o[3]) && is_ints(&o[4], at::kLong) && is_ints(&o[5]),
+            "out must be contiguous int32 tensors (positions int64)");
+    REQUIRE(buffer_rows >= b && buffer_rows <= kMost && o[0].numel() == buffer_rows + 1 && o[1].numel() == buffer_rows + 1 && o[3].numel() == num_tokens &&
+                o[4].numel() == num_tokens && o[5].dim() == 2 && o[5].size(0) >= b && o[5].size(1) == cols,
+            "out does not fit the step");
+    REQUIRE(!parents || (is_ints(&o[6], at::kLong) && o[6].dim() == 2 && o[6].size(0) == num_tokens && o[6].size(1) == words),
+            "tree_masks must be int64 (tokens, mask_words)");
+  }
+  LAUNCH(b200_step_tables(ints(rows), ints(cached), ints(fresh), ints(parents), static_cast<int32_t>(b), num_tokens, block_size, ints(t[0]),
+                          table_stride(*t[0]), static_cast<int32_t>(cols), static_cast<int32_t>(t[0]->size(0)), ints(t[1]), ints(t[2]),
+                          ints(t[3]), t[2]->numel(), static_cast<int32_t>(buffer_rows), ints(&o[0]), ints(&o[1]), ints(&o[2]), ints(&o[3]),
+                          longs(&o[4]), ints(&o[5]), parents ? reinterpret_cast<uint64_t*>(longs(&o[6])) : nullptr, words, stream_ptr()));
+  PyObject* res = PyTuple_New(7);
+  if (!res) return nullptr;
+  for (int i = 0; i < 7; ++i) {
+    if (i == 6 && !parents) {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(res, i, Py_None);
+    } else {
+      PyTuple_SET_ITEM(res, i, THPVariable_Wrap(std::move(o[i])));
+    }
+  }
+  return res;
+  END_HANDLE_TH_ERRORS
+}
+
+// release_blocks(tables, owned, free_blocks, pool, block_size, rows, keep_lens); rows may be None.
+PyObject* py_release_blocks(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(7, "release_blocks");
+  const Tensor *t[4], *rows, *keep;
+  static const char* names[4] = {"tables", "owned", "free_blocks", "pool"};
+  for (int i = 0; i < 4; ++i)
+    if (!(t[i] = tensor_of(a[i], names[i]))) return nullptr;
+  int block_size;
+  if (!as_int(a[4], &block_size) || !optional_tensor(a[5], "rows", &rows) || !(keep = tensor_of(a[6], "keep_lens"))) return nullptr;
+  if (!all_cuda({t[0], t[1], t[2], t[3], rows, keep}) || !same_device(*t[0], {t[1], t[2], t[3], rows, keep}) ||
+      !check_block_state(*t[0], *t[1], *t[2], *t[3]))
+    return nullptr;
+  const int64_t b = keep->numel();
+  REQUIRE(is_ints(keep) && keep->dim() == 1, "keep_lens must be int32, one per sequence");
+  REQUIRE(b <= kMost && (rows ? is_ints(rows) && rows->dim() == 1 && rows->numel() == b : b <= t[0]->size(0)), "rows must be int32, one per sequence");
+  const c10::cuda::CUDAGuard guard(t[0]->device());
+  LAUNCH(b200_release_blocks(ints(rows), ints(keep), static_cast<int32_t>(b), block_size, ints(t[0]), table_stride(*t[0]),
+                             static_cast<int32_t>(t[0]->size(1)), static_cast<int32_t>(t[0]->size(0)), ints(t[1]), ints(t[2]), ints(t[3]),
+                             t[2]->numel(), stream_ptr()));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// The workspace is a call's own, out of torch's allocator: two graphs that hold such calls, or two streams, share none.
+PyObject* do_tree(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& cu, const Tensor& lens, const Tensor& bt,
+                  const Tensor* masks, double scale, int hkv, Tensor* result) {
+  if (q.dim() != 3) {
+    PyErr_SetString(PyExc_ValueError, "tree_attention: q must be (tokens, heads, head_dim)");
+    return nullptr;
+  }
+  if (!all_cuda({&q, &kc, &vc, &cu, &lens, &bt, masks}) || !same_device(q, {&kc, &vc, &cu, &lens, &bt, masks})) return nullptr;
+  const int64_t n = q.size(0), h = q.size(1), d = q.size(2), b = lens.numel();
+  REQUIRE(q.scalar_type() == at::kBFloat16 && kc.scalar_type() == at::kBFloat16 && vc.scalar_type() == at::kBFloat16, "q and caches must be bf16");
+  REQUIRE((d <= 1 || q.stride(2) == 1) && (h <= 1 || q.stride(1) == d), "query heads must be contiguous");
+  REQUIRE(kc.dim() == 4 && kc.is_contiguous() && vc.is_contiguous() && vc.sizes() == kc.sizes() && kc.size(2) == hkv && kc.size(3) == d,
+          "caches must be contiguous (blocks, block size, kv heads, head_dim)");
+  REQUIRE(is_ints(&lens) && lens.dim() == 1 && is_ints(&cu) && cu.dim() == 1 && cu.numel() == b + 1, "context_lens and cu_seqlens_q must be int32, one and one more than the sequences");
+  REQUIRE(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) >= b && (bt.size(1) <= 1 || bt.stride(1) == 1), "block_tables must be int32 with contiguous rows, one per sequence");
+  REQUIRE(!masks || (is_ints(masks, at::kLong) && masks->dim() == 2 && masks->size(0) == n), "tree_masks must be int64 (tokens, mask_words)");
+  REQUIRE(n <= kMost && h <= kMost && b <= kMost && kc.size(1) <= kMost && bt.size(1) <= kMost && (!masks || masks->size(1) <= 4), "too large");
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out = empty_like_rows({n, h, d}, q);
+  if (n > 0 && b > 0) {
+    const int64_t bytes = b200_tree_workspace_bytes(static_cast<int>(h), hkv, static_cast<int>(d));
+    if (bytes < 0) return raise_status(static_cast<int>(bytes));
+    const Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, q.device(), std::nullopt);
+    LAUNCH(b200_tree_attn(q.data_ptr(), n > 1 ? q.stride(0) : h * d, kc.data_ptr(), vc.data_ptr(), kc.size(0), static_cast<int32_t>(kc.size(1)), ints(&bt),
+                          table_stride(bt), static_cast<int32_t>(bt.size(1)), ints(&cu), ints(&lens),
+                          // (masks of no words have no address; the library refuses them by their width)
+                          masks ? static_cast<const uint64_t*>(masks->numel() ? masks->data_ptr() : ws.data_ptr()) : nullptr, masks ? static_cast<int32_t>(masks->size(1)) : 0,
+                          out.data_ptr(), ws.data_ptr(), bytes, static_cast<int32_t>(b), static_cast<int32_t>(n), static_cast<int32_t>(h), hkv,
+                          static_cast<int32_t>(d), static_cast<float>(scale), stream_ptr()));
+  }
+  *result = std::move(out);
+  return kFine;
+}
+
+// tree_attention(q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_masks, scale, num_kv_heads); tree_masks may be None.
+PyObject* py_tree_attention(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(9, "tree_attention");
+  const Tensor *t[6], *masks;
+  static const char* names[6] = {"q", "k_cache", "v_cache", "cu_seqlens_q", "context_lens", "block_tables"};
+  for (int i = 0; i < 6; ++i)
+    if (!(t[i] = tensor_of(a[i], names[i]))) return nullptr;
+  double scale;
+  int hkv;
+  if (!optional_tensor(a[6], "tree_masks", &masks) || !as_double(a[7], &scale) || !as_int(a[8], &hkv)) return nullptr;
+  Tensor out;
+  if (!do_tree(*t[0], *t[1], *t[2], *t[3], *t[4], *t[5], masks, scale, hkv, &out)) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// accept_tree(draft_tokens, target_tokens, parents, cu_seqlens_q, cached_lens, context_lens, max_path) ->
+// (accepted, path, tokens, new cached_lens)
+PyObject* py_accept_tree(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(7, "accept_tree");
+  const Tensor* t[6];
+  static const char* names[6] = {"draft_tokens", "target_tokens", "parents", "cu_seqlens_q", "cached_lens", "context_lens"};
+  for (int i = 0; i < 6; ++i)
+    if (!(t[i] = tensor_of(a[i], names[i]))) return nullptr;
+  int max_path;
+  if (!as_int(a[6], &max_path)) return nullptr;
+  if (!all_cuda({t[0], t[1], t[2], t[3], t[4], t[5]}) || !same_device(*t[0], {t[1], t[2], t[3], t[4], t[5]})) return nullptr;
+  const int64_t n = t[0]->numel(), b = t[4]->numel();
+  REQUIRE(is_ints(t[0], at::kLong) && is_ints(t[1], at::kLong) && t[1]->numel() == n && is_ints(t[2]) && t[2]->numel() == n,
+          "draft_tokens and target_tokens must be int64, parents int32, one per node");
+  REQUIRE(is_ints(t[3]) && t[3]->numel() == b + 1 && is_ints(t[4]) && is_ints(t[5]) && t[5]->numel() == b,
+          "cu_seqlens_q, cached_lens and context_lens must be int32, one per sequence (cu_seqlens_q one more)");
+  REQUIRE(max_path >= 1 && n <= kMost && b <= kMost, "max_path must be at least 1");
+  const c10::cuda::CUDAGuard guard(t[0]->device());
+  const auto dev = t[0]->device();
+  Tensor o[4] = {at::detail::empty_cuda({b}, at::kInt, dev, std::nullopt), at::detail::empty_cuda({b, max_path}, at::kInt, dev, std::nullopt),
+                 at::detail::empty_cuda({b, max_path}, at::kLong, dev, std::nullopt), at::detail::empty_cuda({b}, at::kInt, dev, std::nullopt)};
+  LAUNCH(b200_accept_tree(longs(t[0]), longs(t[1]), ints(t[2]), ints(t[3]), ints(t[4]), ints(t[5]), static_cast<int32_t>(b),
+                          static_cast<int32_t>(n), max_path, ints(&o[0]), ints(&o[1]), longs(&o[2]), ints(&o[3]), stream_ptr()));
+  PyObject* res = PyTuple_New(4);
+  if (!res) return nullptr;
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(res, i, THPVariable_Wrap(std::move(o[i])));
+  return res;
+  END_HANDLE_TH_ERRORS
+}
+
+// compact_kvcache(kv_cache, path, accepted, start_lens, block_tables)
+PyObject* py_compact_kvcache(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(5, "compact_kvcache");
+  const Tensor* t[5];
+  static const char* names[5] = {"kv_cache", "path", "accepted", "start_lens", "block_tables"};
+  for (int i = 0; i < 5; ++i)
+    if (!(t[i] = tensor_of(a[i], names[i]))) return nullptr;
+  const Tensor &cache = *t[0], &path = *t[1], &bt = *t[4];
+  if (!all_cuda({t[0], t[1], t[2], t[3], t[4]}) || !same_device(cache, {t[1], t[2], t[3], t[4]})) return nullptr;
+  REQUIRE(cache.dim() >= 4 && cache.is_contiguous(), "kv_cache must be contiguous (..., blocks, block size, kv heads, head_dim)");
+  const int64_t b = t[2]->numel(), dims = cache.dim(), row = cache.size(dims - 1) * cache.size(dims - 2) * cache.element_size();
+  const int64_t plane = cache.size(dims - 4) * cache.size(dims - 3) * row, planes = plane > 0 ? cache.numel() * cache.element_size() / plane : 0;
+  REQUIRE(is_ints(&path) && path.dim() == 2 && path.size(0) == b && is_ints(t[2]) && is_ints(t[3]) && t[3]->numel() == b,
+          "path must be int32 (sequences, nodes), accepted and start_lens int32, one per sequence");
+  REQUIRE(bt.scalar_type() == at::kInt && bt.dim() == 2 && bt.size(0) >= b && (bt.size(1) <= 1 || bt.stride(1) == 1), "block_tables must be int32 with contiguous rows, one per sequence");
+  REQUIRE(b <= kMost && path.size(1) <= kMost && bt.size(1) <= kMost && planes <= kMost && cache.size(dims - 3) <= kMost, "too large");
+  const c10::cuda::CUDAGuard guard(cache.device());
+  if (b > 0 && planes > 0)
+    LAUNCH(b200_compact_kvcache(cache.data_ptr(), static_cast<int32_t>(planes), plane, row, cache.size(dims - 4), static_cast<int32_t>(cache.size(dims - 3)),
+                                ints(&path), static_cast<int32_t>(path.size(1)), ints(t[2]), ints(t[3]), ints(&bt), table_stride(bt),
+                                static_cast<int32_t>(bt.size(1)), static_cast<int32_t>(b), stream_ptr()));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     FAST("store_kvcache", py_store_kvcache),
@@ -580,6 +824,11 @@ PyMethodDef methods[] = {
     FAST("pack_decode", py_pack_decode),
     FAST("upload_record", py_upload_record),
     FAST("unpack_decode_metadata", py_unpack),
+    FAST("step_tables", py_step_tables),
+    FAST("release_blocks", py_release_blocks),
+    FAST("tree_attention", py_tree_attention),
+    FAST("accept_tree", py_accept_tree),
+    FAST("compact_kvcache", py_compact_kvcache),
     {nullptr, nullptr, 0, nullptr},
 };
 

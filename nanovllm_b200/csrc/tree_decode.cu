@@ -1,0 +1,219 @@
+// What a step with drafted trees does behind the model: the walk along the sampled tokens, and the accepted nodes' cache rows to
+// their places.
+#include "../../include/b200_attn.h"
+#include "kernels.cuh"
+
+namespace b200 {
+extern std::atomic<long long> g_launches;
+
+// ---- the walk ------------------------------------------------------------------------------------------------------
+// target[r] is what the target model sampled behind node r, so the path from the root along children whose drafted token equals
+// their parent's sample is made of the target's own samples, at any temperature.  One warp per tree: the nodes' parents and
+// tokens go to shared memory once, and each level is a ballot over the nodes behind the current one.
+constexpr int kAcceptWarps = 4;
+constexpr int kAcceptNodes = 256;        // nodes of a tree that are kept in shared memory; later ones are read where they lie
+
+struct AcceptParams {
+  const long long *draft, *target;
+  const int *parents, *cu, *cached, *context;
+  int batch, num_tokens, max_path;
+  int *accepted, *path, *cached_out;
+  long long* tokens;
+};
+
+__global__ void __launch_bounds__(kAcceptWarps * 32) accept_tree_kernel(const AcceptParams p) {
+  __shared__ long long s_draft[kAcceptWarps][kAcceptNodes], s_target[kAcceptWarps][kAcceptNodes];
+  __shared__ int s_parent[kAcceptWarps][kAcceptNodes];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i = blockIdx.x * kAcceptWarps + warp;
+  if (i >= p.batch) return;
+  const int start = max(0, min(p.cu[i], p.num_tokens)), nodes = max(0, min(p.cu[i + 1], p.num_tokens) - start);
+  const int cached = p.cached[i];
+  int count = 0;
+  if (p.context[i] > 0 && nodes > 0) {
+    for (int n = lane; n < min(nodes, kAcceptNodes); n += 32) {
+      s_draft[warp][n] = p.draft[start + n];
+      s_target[warp][n] = p.target[start + n];
+      s_parent[warp][n] = p.parents[start + n];
+    }
+    __syncwarp();
+    int cur = 0;
+    while (true) {
+      const long long want = cur < kAcceptNodes ? s_target[warp][cur] : p.target[start + cur];
+      if (lane == 0) {
+        p.path[static_cast<long long>(i) * p.max_path + count] = cur;
+        p.tokens[static_cast<long long>(i) * p.max_path + count] = want;
+      }
+      if (++count == p.max_path) break;
+      int next = -1;
+      for (int base = (cur + 1) & ~31; base < nodes; base += 32) {       // children come behind their parent
+        const int n = base + lane;
+        bool hit = false;
+        if (n > cur && n < nodes)
+          hit = n < kAcceptNodes ? s_parent[warp][n] == cur && s_draft[warp][n] == want
+                                 : p.parents[start + n] == cur && p.draft[start + n] == want;
+        const unsigned found = __ballot_sync(0xffffffffu, hit);
+        if (found) {
+          next = base + __ffs(found) - 1;
+          break;
+        }
+      }
+      if (next < 0) break;
+      cur = next;
+    }
+  }
+  for (int k = count + lane; k < p.max_path; k += 32) {
+    p.path[static_cast<long long>(i) * p.max_path + k] = -1;
+    p.tokens[static_cast<long long>(i) * p.max_path + k] = -1;
+  }
+  if (lane == 0) {
+    p.accepted[i] = count;
+    p.cached_out[i] = cached + count;
+  }
+}
+
+// ---- the cache ------------------------------------------------------------------------------------------------------
+// Row start + path[k] of every plane goes to start + k.  Entries below their place (path[k] < k) are not moved, so a row that is
+// written (k) is read by later moves only where path[k'] = k < k', which that excludes: a thread may have the loads of
+// several moves in flight, and keeps to one 16-byte column of a row.
+constexpr int kCompactThreads = 256;
+constexpr int kCompactPath = 256;        // entries of a path that are looked at together
+
+struct CompactParams {
+  char* cache;
+  long long plane_stride, row_bytes;
+  int planes, vecs;                      // vecs: 16-byte columns of a row
+  long long columns;                     // planes * vecs
+  int num_blocks, block_size;
+  const int *path, *accepted, *start, *block_tables;
+  int path_cols;
+  long long bt_row_stride;
+  int bt_cols;
+};
+
+__device__ __forceinline__ long long compact_row(const CompactParams& p, const int* table, int at) {
+  const int col = at / p.block_size;
+  if (at < 0 || col >= p.bt_cols) return -1;
+  const int id = table[col];
+  return id >= 0 && id < p.num_blocks ? static_cast<long long>(id) * p.block_size + (at - col * p.block_size) : -1;
+}
+
+__global__ void __launch_bounds__(kCompactThreads) compact_kvcache_kernel(const CompactParams p) {
+  __shared__ long long s_src[kCompactPath], s_dst[kCompactPath];
+  __shared__ int s_moves;
+  const int i = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int* const table = p.block_tables + i * p.bt_row_stride;
+  const long long column = static_cast<long long>(blockIdx.x) * kCompactThreads + tid;
+  char* mine = nullptr;
+  if (column < p.columns) {
+    const long long plane = column / p.vecs;
+    mine = p.cache + plane * p.plane_stride + (column - plane * p.vecs) * 16;
+  }
+  const int n = min(p.accepted[i], p.path_cols), start = p.start[i];
+  for (int base = 0; base < n; base += kCompactPath) {
+    if (tid < 32) {
+      int moves = 0;
+      for (int k0 = base; k0 < min(n, base + kCompactPath); k0 += 32) {
+        const int k = k0 + lane;
+        long long src = -1, dst = -1;
+        if (k < n) {
+          const int node = p.path[static_cast<long long>(i) * p.path_cols + k];
+          if (node > k && node <= 0x7fffffff - start) {
+            src = compact_row(p, table, start + node);
+            dst = compact_row(p, table, start + k);
+          }
+        }
+        const bool move = src >= 0 && dst >= 0;
+        const unsigned all = __ballot_sync(0xffffffffu, move);
+        if (move) {
+          const int at = moves + __popc(all & ((1u << lane) - 1));
+          s_src[at] = src * p.row_bytes;
+          s_dst[at] = dst * p.row_bytes;
+        }
+        moves += __popc(all);
+      }
+      if (lane == 0) s_moves = moves;
+    }
+    __syncthreads();
+    const int moves = s_moves;
+    if (mine)
+      for (int k = 0; k < moves; k += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k + u < moves) v[u] = *reinterpret_cast<const uint4*>(mine + s_src[k + u]);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (k + u < moves) *reinterpret_cast<uint4*>(mine + s_dst[k + u]) = v[u];
+      }
+    __syncthreads();
+  }
+}
+
+}  // namespace b200
+
+extern "C" int b200_accept_tree(const int64_t* draft_tokens, const int64_t* target_tokens, const int32_t* parents,
+                                const int32_t* cu_seqlens_q, const int32_t* cached_lens, const int32_t* context_lens, int32_t batch,
+                                int32_t num_tokens, int32_t max_path, int32_t* accepted, int32_t* path, int64_t* tokens,
+                                int32_t* new_cached_lens, void* stream) {
+  using namespace b200;
+  if (batch < 0 || num_tokens < 0 || max_path < 1) return set_error(kErrBadShape, "accept_tree: batch (%d) and num_tokens (%d) must not be negative, max_path (%d) at least 1", batch, num_tokens, max_path);
+  if (batch == 0) return kOk;
+  if (!cu_seqlens_q || !cached_lens || !context_lens || !accepted || !path || !tokens || !new_cached_lens ||
+      (num_tokens > 0 && (!draft_tokens || !target_tokens || !parents)))
+    return set_error(kErrNullPointer, "accept_tree: null pointer argument");
+  if ((reinterpret_cast<uintptr_t>(draft_tokens) | reinterpret_cast<uintptr_t>(target_tokens) | reinterpret_cast<uintptr_t>(tokens)) & 7)
+    return set_error(kErrMisaligned, "accept_tree: tokens must be 8-byte aligned");
+  AcceptParams p;
+  p.draft = reinterpret_cast<const long long*>(draft_tokens);
+  p.target = reinterpret_cast<const long long*>(target_tokens);
+  p.parents = parents;
+  p.cu = cu_seqlens_q;
+  p.cached = cached_lens;
+  p.context = context_lens;
+  p.batch = batch;
+  p.num_tokens = num_tokens;
+  p.max_path = max_path;
+  p.accepted = accepted;
+  p.path = path;
+  p.cached_out = new_cached_lens;
+  p.tokens = reinterpret_cast<long long*>(tokens);
+  accept_tree_kernel<<<(batch + kAcceptWarps - 1) / kAcceptWarps, kAcceptWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  g_launches.fetch_add(1);
+  return check_cuda(cudaGetLastError(), "accept_tree launch");
+}
+
+extern "C" int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_stride_bytes, int64_t row_bytes, int64_t num_blocks,
+                                    int32_t block_size, const int32_t* path, int32_t path_cols, const int32_t* accepted,
+                                    const int32_t* start_lens, const int32_t* block_tables, int64_t bt_row_stride, int32_t bt_cols,
+                                    int32_t batch, void* stream) {
+  using namespace b200;
+  if (batch < 0 || batch > 65535 || planes < 0 || path_cols < 0) return set_error(kErrBadShape, "compact_kvcache: batch must be in [0, 65535], planes and path_cols not negative (got %d, %d, %d)", batch, planes, path_cols);
+  if (batch == 0 || planes == 0 || path_cols <= 1) return kOk;
+  if (!cache || !path || !accepted || !start_lens || !block_tables) return set_error(kErrNullPointer, "compact_kvcache: null pointer argument");
+  if (block_size <= 0 || num_blocks <= 0 || num_blocks * block_size >= (1LL << 31)) return set_error(kErrBadShape, "compact_kvcache: num_blocks * block_size must be in (0, 2^31)");
+  if (bt_cols <= 0 || bt_row_stride < bt_cols) return set_error(kErrBadShape, "compact_kvcache: bad block table geometry");
+  if (row_bytes <= 0 || row_bytes > (1 << 20) || plane_stride_bytes < num_blocks * block_size * row_bytes) return set_error(kErrBadShape, "compact_kvcache: rows of 1 to 2^20 bytes, planes that do not overlap");
+  if ((reinterpret_cast<uintptr_t>(cache) | row_bytes | plane_stride_bytes) & 15) return set_error(kErrMisaligned, "compact_kvcache: cache, rows and planes must be multiples of 16 bytes");
+  CompactParams p;
+  p.cache = static_cast<char*>(cache);
+  p.plane_stride = plane_stride_bytes;
+  p.row_bytes = row_bytes;
+  p.planes = planes;
+  p.vecs = static_cast<int>(row_bytes / 16);
+  p.columns = static_cast<long long>(planes) * p.vecs;
+  p.num_blocks = static_cast<int>(num_blocks);
+  p.block_size = block_size;
+  p.path = path;
+  p.accepted = accepted;
+  p.start = start_lens;
+  p.block_tables = block_tables;
+  p.path_cols = path_cols;
+  p.bt_row_stride = bt_row_stride;
+  p.bt_cols = bt_cols;
+  const long long blocks = (p.columns + kCompactThreads - 1) / kCompactThreads;
+  if (blocks > 0x7fffffffLL) return set_error(kErrBadShape, "compact_kvcache: too many planes");
+  compact_kvcache_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch)), kCompactThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  g_launches.fetch_add(1);
+  return check_cuda(cudaGetLastError(), "compact_kvcache launch");
+}

@@ -51,6 +51,16 @@ def prefill_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seq
                                            num_kv_heads, block_tables, kernel_variant)
 
 
+def tree_attention(q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_masks, scale, num_kv_heads):
+    """Attention of a step in which every sequence brings drafted tokens, whose keys and values are in the caches
+    already: q (tokens, H, D) -> (tokens, H, D).  Sequence i's nodes are rows cu_seqlens_q[i] .. cu_seqlens_q[i+1] and the
+    last of its context_lens[i] cached tokens; each sees what lies in front of them and the nodes that its row of
+    tree_masks (tokens, words; int64, bit n: node n) names, or, with tree_masks None, those before it and itself.  Rows
+    outside cu_seqlens_q are not written.  Details: b200_tree_attn in include/b200_attn.h."""
+    return _lib.native().tree_attention(q, k_cache, v_cache, cu_seqlens_q, context_lens, block_tables, tree_masks, scale,
+                                        num_kv_heads)
+
+
 class Attention(nn.Module):
     """Constructor, attributes and forward of the reference module
     (nanovllm/layers/attention.py:43-75); the model runner finds the layer through its
@@ -67,5 +77,11 @@ class Attention(nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, already_stored: bool = False):
         """`already_stored` is not part of the reference's signature: the fused producer kernel
         (layers/qk_norm_rope.py) has written k and v to the cache and passes True."""
-        return _lib.native().attention_forward(q, k, v, self.k_cache, self.v_cache, _context_getter(), self.scale,
-                                               self.num_kv_heads, already_stored)
+        context = _context_getter()
+        if type(context) is _own_context.TreeContext:
+            if not already_stored:
+                store_kvcache(k, v, self.k_cache, self.v_cache, context.slot_mapping)
+            return tree_attention(q, self.k_cache, self.v_cache, context.cu_seqlens_q, context.context_lens, context.block_tables,
+                                  context.tree_masks, self.scale, self.num_kv_heads)
+        return _lib.native().attention_forward(q, k, v, self.k_cache, self.v_cache, context, self.scale, self.num_kv_heads,
+                                               already_stored)

@@ -22,6 +22,14 @@ class Context:
     block_tables: torch.Tensor | None = None
 
 
+@dataclass
+class TreeContext(Context):
+    """A step in which every sequence brings drafted tokens (not in the reference): sequence i's are rows cu_seqlens_q[i] ..
+    cu_seqlens_q[i+1], the last of its context_lens[i] tokens; tree_masks says which of them each sees (None: a chain).
+    Inside nano-vllm, put such a record where its get_context() looks (nanovllm.utils.context._CONTEXT)."""
+    tree_masks: torch.Tensor | None = None
+
+
 _CONTEXT = Context()
 
 
@@ -34,6 +42,12 @@ def set_context(is_prefill, cu_seqlens_q=None, cu_seqlens_k=None, max_seqlen_q=0
     global _CONTEXT
     _CONTEXT = Context(is_prefill, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k,
                        slot_mapping, context_lens, block_tables)
+
+
+def set_tree_context(cu_seqlens_q, context_lens, slot_mapping, block_tables, tree_masks=None):
+    global _CONTEXT
+    _CONTEXT = TreeContext(False, cu_seqlens_q=cu_seqlens_q, slot_mapping=slot_mapping, context_lens=context_lens,
+                           block_tables=block_tables, tree_masks=tree_masks)
 
 
 def reset_context():
