@@ -24,6 +24,7 @@
 // TMEM: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512).  Every mbarrier wait is bounded.
 #include "../../include/b200_attn.h"
 #include "kernels.cuh"
+#include "tc_wait.cuh"
 #include "tcgen05.cuh"
 
 #include <type_traits>
@@ -50,8 +51,8 @@ static __device__ int g_status_prefill_tc2 = 0;
 
 static __device__ unsigned int g_prefill_ticket = 0;
 
-// The kernel's bounded waits.  Six roles run through their loops at the same time and share the SM's instruction cache, so code
-// size is time here.  Us for 256 prompts of 100 .. 1024 tokens with the store | without it, 256 of 10 .. 300 without it, in four launches
+// The bounded waits are those of tc_wait.cuh.  Six roles run through their loops at the same time and share the SM's
+// instruction cache, so code size is time here.  Us for 256 prompts of 100 .. 1024 tokens with the store | without it, 256 of 10 .. 300 without it, in four launches
 // after a rest (in 300 launches on end, at the power cap):
 //   mbar_wait() (64-bit clock arithmetic and a spin counter at each of some thirty places), output and rescaling
 //     loops unrolled, a mask by comparisons                                 803 | 657, 167  (885 | 766, 185)
@@ -59,42 +60,6 @@ static __device__ unsigned int g_prefill_ticket = 0;
 //   one output path instead of two, shifts for divisions by powers of two, table columns counted along and one copy
 //     of the store's row loop: 64 KB of code for 78 with the store          653 | 598, 134  (770 | 713, 159)
 // So the store in the launch costs 55 us; a launch of its own in front of the form without it 181 (782 for both, 884 on end).
-//
-// How long the hardware suspends a failed test is its own affair, so a count of tests is a limit but not one in time.  The time
-// limit is the producer's, on the low word of the clock: it sets the abort flag, which every other wait looks at after a
-// failed test.  That bounds them all: whatever hangs stops the ring that the producer waits for, and at the end the producer
-// waits until every role has taken the end marker, which it does when it is through with all items.
-constexpr int kT2WaitLimit = 1 << 22;
-__device__ __forceinline__ bool t2_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-#pragma unroll 1
-  for (int n = 0; n < kT2WaitLimit; ++n) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (*abort_flag) return false;
-  }
-  *abort_flag = 1;
-  return false;
-}
-__device__ __forceinline__ uint32_t t2_clock() {
-  uint32_t c;
-  asm volatile("mov.u32 %0, %%clock;" : "=r"(c));
-  return c;
-}
-__device__ __forceinline__ bool t2_wait_timed(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  const uint32_t t0 = t2_clock();
-#pragma unroll 1
-  while (!mbar_try_wait(bar, parity)) {
-    if (*abort_flag) return false;
-    if (t2_clock() - t0 > static_cast<uint32_t>(kSpinLimitCycles)) {
-      *abort_flag = 1;
-      return false;
-    }
-  }
-  return true;
-}
-// On the S -> softmax -> PV chain: the second test does not come behind a look at the flag (long sequences lose 3 % to it).
-__device__ __forceinline__ bool t2_wait_hot(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  return mbar_try_wait(bar, parity) || t2_wait(bar, parity, abort_flag);
-}
 
 struct T2Item {
   int seq;        // -1: no more work

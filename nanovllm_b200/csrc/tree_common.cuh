@@ -20,6 +20,8 @@ struct TreeParams {
   int mask_words;                    // 32-bit words of a row
   int batch, total_q, H, Hkv, G;
   float scale_log2;
+  int* pieces;                       // [2 * CTAs] records of cut units (TreePiece)
+  float* partials;                   // [2 * CTAs] partial results
 };
 
 // Which of 32 keys a row sees.  `d`: index of the first of them among the step's nodes (negative: that many lie in front of
