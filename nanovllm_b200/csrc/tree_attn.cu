@@ -8,13 +8,19 @@
 // One persistent CTA per SM.  A unit is (sequence, block of up to 2 * QT nodes, kv head), QT = 128 / G.  All units' key tiles (128
 // keys) stand in one line, which is cut into equal shares, one per CTA; a unit that a cut runs through leaves partial
 // results (maximum, sum, unnormalised output in fp32), which a second kernel joins in order.  Roles of the 16 warps:
-//   warp 0        TMA producer: walks the CTA's share, publishes items, loads Q tiles and a ring of K and V tiles
-//   warp 1        one thread issues tcgen05.mma: S_X = Q_X K^T, O_X += P_X V (P read from TMEM)
-//   warps 4-7, 8-11   softmax warpgroups of the halves A and B: a thread owns a row; P goes back over S
+//   warps 0, 3    a thread each loads through TMA: 0 walks the CTA's share, publishes items, loads Q tiles and a ring of K tiles,
+//                 3 a ring of V tiles
+//   warps 1, 2    a thread each issues tcgen05.mma: 1 S_X = Q_X K^T, 2 O_X += P_X V (P read from TMEM)
+//   warps 4-7, 8-11   softmax warpgroups of the halves A and B: a thread owns a row
 //   warps 12-15   output warpgroup: finished accumulators out of TMEM, to `out` or to the partials
-// The halves are the two chains S -> softmax -> P V that TMEM has room for.  Up to 128 rows, they take the key tiles of a unit in
-// turn and the output warpgroup joins them; with more, each has a Q tile of its own and both use every key tile.
-// TMEM: S_A [0,128)  S_B [128,256)  O_A [256,384)  O_B [384,512).  Every mbarrier wait is bounded.
+// The halves are two softmax chains.  Work is a row of steps that they take in strict turn, across the units' borders: a step is a
+// key tile of a unit with at most 128 rows (the output warpgroup joins what the halves have of it), or a key tile for one of the
+// two Q tiles of a larger unit.
+// TMEM: S [0,128)  P_A [128,192)  P_B [192,256)  O_A [256,384)  O_B [384,512).  Both halves' scores go through one S: a row is in
+// its thread's registers 200 cycles after the product, and then the next step's product may run.  With an S of its own in
+// which P replaced the scores, a half's next S had to wait for its P V: a chain of 3740 cycles a tile at 256 rows, of which the
+// softmax is 1990.
+// Every mbarrier wait is bounded.
 #include <atomic>
 
 #include "../../include/b200_attn.h"
@@ -29,11 +35,11 @@ constexpr int kTrKv = 128;
 constexpr int kTrSub = 128 * 128;             // one 64-column sub-tile of a 128-row tile (bytes)
 constexpr int kTrTile = 2 * kTrSub;           // 128 rows x 128 dims bf16 = 32 KiB
 constexpr int kTrThreads = 512;
-constexpr int kTrRing = 5;                    // K and V tiles, one ring in the order in which they are used
+constexpr int kTrRingK = 2, kTrRingV = 3;     // tiles of K and V in shared memory
 constexpr int kTrItems = 4;                   // items in flight
 constexpr float kTrRescale = 8.0f;
 // The line's measure: cost of a key tile with the halves sharing it out, with a Q tile each, and of a unit by itself.
-constexpr int kTrCostSplit = 4, kTrCostPair = 5, kTrCostUnit = 3;
+constexpr int kTrCostSplit = 4, kTrCostPair = 5, kTrCostUnit = 10;
 // Partial results of one piece: 8 groups of 32 rows, each [128 dims][32 rows] and [max, sum][32 rows] in fp32, so that both kernels
 // move whole lines with a row per lane.
 constexpr int kTrGroup = 130 * 32;
@@ -48,9 +54,16 @@ struct TreeItem {
   int node0, nodes;     // that node's index in its sequence, and how many the unit has
   int first, Lk;        // position of the sequence's node 0; its keys
   int t0, n;            // key tiles of this piece
-  int split;            // the halves share the key tiles out
+  int split;            // at most QT nodes: a step per key tile, else two
+  int turn;             // the half that takes the unit's first step
   int partial;          // -1: the whole unit, else where its partial results go
 };
+
+// 1-D bulk copy global -> shared, completion counted on an mbarrier (addresses and size multiples of 16).
+__device__ __forceinline__ void tree_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
 
 // What a cut unit's pieces are: a record for each place of partial results, written by every CTA.
 struct TreePiece {
@@ -73,23 +86,64 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int QT, int i) 
   s.last_split = s.nodes - (s.blocks - 1) * 2 * QT <= QT;
   return s;
 }
-__device__ __forceinline__ long long tree_cost(const TreeSeq& s, int Hkv) {
+// (32 bits: the host refuses geometries whose line might be longer)
+__device__ __forceinline__ unsigned tree_cost(const TreeSeq& s, int Hkv) {
   if (s.blocks == 0) return 0;
-  return Hkv * (static_cast<long long>(s.blocks) * (s.tiles * kTrCostPair + kTrCostUnit) -
-                (s.last_split ? static_cast<long long>(s.tiles) * (kTrCostPair - kTrCostSplit) : 0));
+  return Hkv * (s.blocks * (s.tiles * kTrCostPair + kTrCostUnit) - (s.last_split ? s.tiles * (kTrCostPair - kTrCostSplit) : 0));
 }
 // Place `off` of a sequence's part of the line: unit (block * Hkv + head) and key tile.
-__device__ __forceinline__ void tree_locate(const TreeSeq& s, int Hkv, long long off, int& unit, int& tile) {
-  const long long pair = static_cast<long long>(s.tiles) * kTrCostPair + kTrCostUnit;
-  const long long block = min(off / (pair * Hkv), static_cast<long long>(s.blocks - 1));
+__device__ __forceinline__ void tree_locate(const TreeSeq& s, int Hkv, unsigned off, int& unit, int& tile) {
+  const unsigned pair = s.tiles * kTrCostPair + kTrCostUnit;
+  const unsigned block = s.blocks == 1 ? 0 : min(off / (pair * Hkv), static_cast<unsigned>(s.blocks - 1));
   off -= block * pair * Hkv;
-  const int w = block == s.blocks - 1 && s.last_split ? kTrCostSplit : kTrCostPair;
-  const long long one = static_cast<long long>(s.tiles) * w + kTrCostUnit;
-  const long long h = off / one;
+  const unsigned w = block == s.blocks - 1 && s.last_split ? kTrCostSplit : kTrCostPair;
+  const unsigned one = s.tiles * w + kTrCostUnit;
+  const unsigned h = off / one;
   off -= h * one;
   unit = static_cast<int>(block * Hkv + h);
-  tile = static_cast<int>(max(off - kTrCostUnit, 0LL) / w);
+  tile = static_cast<int>(off < kTrCostUnit ? 0 : (off - kTrCostUnit) / w);
 }
+
+// A key tile of K or V into its place: in one box per half of the dims; of a sequence's last tile only what it has (`left` keys), in
+// boxes of 16 rows.
+__device__ __forceinline__ void tree_load(const CUtensorMap* whole, const CUtensorMap* map16, uint64_t* full, unsigned char* dst, int h, int row,
+                                          int left) {
+  if (left > kTrKv - 16) {
+    mbar_expect_tx(full, kTrTile);
+    tma_load_3d(dst, whole, full, 0, h, row);
+    tma_load_3d(dst + kTrSub, whole, full, 64, h, row);
+    return;
+  }
+  const int boxes = (left + 15) >> 4;
+  mbar_expect_tx(full, boxes * 4096);
+#pragma unroll 1
+  for (int b = 0; b < boxes; ++b) {
+    tma_load_3d(dst + b * 2048, map16, full, 0, h, row + b * 16);
+    tma_load_3d(dst + kTrSub + b * 2048, map16, full, 64, h, row + b * 16);
+  }
+}
+// Walks along a sequence's key tiles: the cache row of each, far below zero (TMA reads zeros there) where its block is none of
+// the cache.
+struct TreeRows {
+  const int* blocks;
+  int row, in_block;
+  __device__ __forceinline__ void start(const TreeParams& p, int seq, int tile) {
+    const int col = tile * kTrKv / p.block_size;
+    blocks = p.block_tables + seq * p.bt_row_stride + col;
+    in_block = -(tile * kTrKv - col * p.block_size);        // (not looked up yet)
+  }
+  __device__ __forceinline__ int next(const TreeParams& p) {
+    if (in_block <= 0) {
+      const int blk = __ldg(blocks++);
+      row = blk >= 0 && blk < p.num_blocks ? blk * p.block_size - in_block : -(1 << 30);
+      in_block += p.block_size;
+    }
+    const int r = row;
+    row += kTrKv;
+    in_block -= kTrKv;
+    return r;
+  }
+};
 
 __global__ void __launch_bounds__(kTrThreads, 1)
 tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -97,34 +151,41 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
                  const __grid_constant__ CUtensorMap map_v16) {
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* const sQ = smem;                      // [2][32 KiB]
-  unsigned char* const sKV = smem + 2 * kTrTile;       // [kTrRing][32 KiB]
+  unsigned char* const sK = smem + 2 * kTrTile;        // [kTrRingK][32 KiB]
+  unsigned char* const sV = sK + kTrRingK * kTrTile;   // [kTrRingV][32 KiB]
   __shared__ __align__(8) uint64_t bar_item_full[kTrItems], bar_item_empty[kTrItems];
-  __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_empty[2], bar_kv_full[kTrRing], bar_kv_empty[kTrRing];
-  __shared__ __align__(8) uint64_t bar_s_full[2], bar_p_full[2], bar_o_final[2], bar_o_free[2], bar_l_full[2], bar_l_empty[2];
+  __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_empty[2];
+  __shared__ __align__(8) uint64_t bar_k_full[kTrRingK], bar_k_empty[kTrRingK], bar_v_full[kTrRingV], bar_v_empty[kTrRingV];
+  __shared__ __align__(8) uint64_t bar_s_full[2], bar_s_free, bar_p_full[2], bar_pv[2], bar_o_final[2], bar_o_free[2], bar_l_full[2], bar_l_empty[2];
   __shared__ float s_max[2][128], s_sum[2][128];       // a half's rows: maximum (log2 units) and sum
   __shared__ __align__(16) TreeItem s_item[kTrItems];
-  __shared__ long long s_scan[kTrThreads / 32];
+  __shared__ unsigned s_scan[kTrThreads / 32];
   __shared__ int s_at[2][3];                           // the share's first place and the one behind its last: sequence, unit, tile
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort, s_bare;                      // s_bare: some sequence has nodes but no keys
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.G, QT = 128 / p.G;
+  // (the join comes in as CTAs of this kernel leave: beside one there is no room)
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     s_abort = 0;
     s_bare = 0;
-    for (int i = 0; i < kTrItems; ++i) { mbar_init(&bar_item_full[i], 1); mbar_init(&bar_item_empty[i], 13); }
+    for (int i = 0; i < kTrItems; ++i) { mbar_init(&bar_item_full[i], 1); mbar_init(&bar_item_empty[i], 15); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar_q_full[i], 1);
       mbar_init(&bar_q_empty[i], 1);
       mbar_init(&bar_s_full[i], 1);
       mbar_init(&bar_p_full[i], 4);
+      mbar_init(&bar_pv[i], 1);
       mbar_init(&bar_o_final[i], 1);
       mbar_init(&bar_o_free[i], 4);
       mbar_init(&bar_l_full[i], 4);
       mbar_init(&bar_l_empty[i], 4);
     }
-    for (int i = 0; i < kTrRing; ++i) { mbar_init(&bar_kv_full[i], 1); mbar_init(&bar_kv_empty[i], 1); }
+    mbar_init(&bar_s_free, 4);
+    for (int i = 0; i < kTrRingK; ++i) { mbar_init(&bar_k_full[i], 1); mbar_init(&bar_k_empty[i], 1); }
+    for (int i = 0; i < kTrRingV; ++i) { mbar_init(&bar_v_full[i], 1); mbar_init(&bar_v_empty[i], 1); }
     mbar_fence_init();
     s_at[0][0] = s_at[1][0] = p.batch;
     s_at[0][1] = s_at[0][2] = s_at[1][1] = s_at[1][2] = 0;
@@ -133,46 +194,47 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   // The CTA's share of the line.  (Lengths ahead of the wait below: no kernel that lets this one start early writes them.)
   // With up to a block of sequences one sum over them gives the total and every sequence's place; larger batches take two.
   {
-    long long total = 0, mine = 0, before = 0;
+    unsigned total = 0;
     TreeSeq s = {};
     const int rounds = (p.batch + kTrThreads - 1) / kTrThreads;
+#pragma unroll 1
     for (int pass = rounds > 1 ? 0 : 1; pass < 2; ++pass) {
-      long long upto = 0, lo = 0, hi = 0;
+      unsigned upto = 0;
+#pragma unroll 1
       for (int r = 0; r < rounds; ++r) {
         const int i = r * kTrThreads + tid;
-        mine = 0;
+        unsigned mine = 0;
         if (i < p.batch) {
           s = tree_seq(p, QT, i);
           mine = tree_cost(s, p.Hkv);
           if (s.nodes > 0 && s.tiles == 0) s_bare = 1;
         }
-        long long x = mine;
+        unsigned x = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const long long y = __shfl_up_sync(0xffffffffu, x, o);
+          const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
           if (lane >= o) x += y;
         }
         if (lane == 31) s_scan[warp] = x;
         __syncthreads();
-        long long all = 0;
-        before = upto;
+        unsigned w = lane < kTrThreads / 32 ? s_scan[lane] : 0;
 #pragma unroll
-        for (int w = 0; w < kTrThreads / 32; ++w) {
-          const long long v = s_scan[w];
-          if (w < warp) before += v;
-          all += v;
+        for (int o = 1; o < kTrThreads / 32; o <<= 1) {
+          const unsigned y = __shfl_up_sync(0xffffffffu, w, o);
+          if (lane >= o) w += y;
         }
-        __syncthreads();
-        before += x - mine;
+        const unsigned all = __shfl_sync(0xffffffffu, w, kTrThreads / 32 - 1), front = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+        const unsigned before = upto + (warp ? front : 0) + x - mine;
         upto += all;
         if (rounds == 1) total = upto;
-        if (pass == 1 && i < p.batch && mine > 0) {
-          lo = total * blockIdx.x / gridDim.x;
-          hi = total * (blockIdx.x + 1) / gridDim.x;
-#pragma unroll
+        else __syncthreads();
+        if (pass == 1 && mine > 0) {
+          // (any function of the CTA that grows from 0 to the total will do)
+          const unsigned one = 0xffffffffu / gridDim.x;
+#pragma unroll 1
           for (int e = 0; e < 2; ++e) {
-            const long long at = e ? hi : lo;
-            if (at >= before && at < before + mine) {
+            const unsigned at = __umulhi(total, one * (blockIdx.x + e));
+            if (at >= before && at < before + mine && blockIdx.x + e < gridDim.x) {
               int unit, tile;
               tree_locate(s, p.Hkv, at - before, unit, tile);
               s_at[e][0] = i;
@@ -186,111 +248,106 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     }
   }
   __syncthreads();
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (s_bare) {
-    // sequences with nodes and no keys: zeros
-    for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
-      const TreeSeq s = tree_seq(p, QT, i);
-      if (s.tiles > 0) continue;
-      uint4* const dst = reinterpret_cast<uint4*>(p.out + static_cast<long long>(s.q_begin) * p.H * 128);
-      for (long long e = tid; e < static_cast<long long>(s.nodes) * p.H * 16; e += kTrThreads) dst[e] = make_uint4(0, 0, 0, 0);
-    }
-  }
-  if (warp == 1) {
-    tc::tmem_alloc(&s_tmem_base, 512);
-    tc::tmem_relinquish();
-  }
-  tc::fence_before_sync();
-  __syncthreads();
-  tc::fence_after_sync();
-  const uint32_t tmem = s_tmem_base;
   volatile int* abort_flag = &s_abort;
+  uint32_t tmem = 0;
+  if (warp > 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (s_bare) {
+      // sequences with nodes and no keys: zeros
+#pragma unroll 1
+      for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
+        const TreeSeq s = tree_seq(p, QT, i);
+        if (s.tiles > 0) continue;
+        uint4* const dst = reinterpret_cast<uint4*>(p.out + static_cast<long long>(s.q_begin) * p.H * 128);
+        for (long long e = tid - 32; e < static_cast<long long>(s.nodes) * p.H * 16; e += kTrThreads - 32) dst[e] = make_uint4(0, 0, 0, 0);
+      }
+    }
+    if (warp == 1) {
+      tc::tmem_alloc(&s_tmem_base, 512);
+      tc::tmem_relinquish();
+    }
+    tc::fence_before_sync();
+    named_bar_sync(1, kTrThreads - 32);         // (the producer is on its way already)
+    tc::fence_after_sync();
+    tmem = s_tmem_base;
+  }
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 80;" ::: "memory");
-    if (warp == 0 && lane == 0) {
-      // ================================ TMA producer ================================
+    if (tid == 0) {
+      // ================================ items, Q and K ================================
       tma_prefetch_desc(&map_q);
       tma_prefetch_desc(&map_k);
       tma_prefetch_desc(&map_v);
       TreePiece pieces[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-      int seq = s_at[0][0], unit = s_at[0][1], t0 = s_at[0][2];
-      const int end_seq = s_at[1][0], end_unit = s_at[1][1], end_tile = s_at[1][2];
-      int n_pub = 0, kv = 0, kv_ph = 1, q_use = 0;
-      bool ok = true;
+      int seq = s_at[0][0], unit = s_at[0][1], from = s_at[0][2], have = -1;
       TreeSeq s = {};
-      int have = -1;
-      while (ok && seq < p.batch && seq <= end_seq) {
+      TreeRows rows = {};
+      const int end_seq = s_at[1][0], end_unit = s_at[1][1], end_tile = s_at[1][2];
+      int n_pub = 0, q_use = 0, turn = 0, k_at = 0, k_ph = 1;
+      bool ok = true, started = false;
+#pragma unroll 1
+      while (ok && seq < p.batch) {
+        // the next unit that has tiles here
         if (have != seq) {
           s = tree_seq(p, QT, seq);
           have = seq;
         }
         if (unit >= s.blocks * p.Hkv) {
-          ++seq;
-          unit = t0 = 0;
+          seq = seq < end_seq ? seq + 1 : p.batch;
+          unit = from = 0;
           continue;
         }
         const bool at_end = seq == end_seq && unit >= end_unit;
-        const int t1 = at_end ? (unit == end_unit ? end_tile : 0) : s.tiles;
-        if (t1 > t0) {
-          const int block = unit / p.Hkv, h = unit - block * p.Hkv, node0 = block * 2 * QT;
-          const int nodes = min(2 * QT, s.nodes - node0), n = t1 - t0;
-          const bool split = nodes <= QT;
-          const bool whole = t0 == 0 && t1 == s.tiles;
-          const int place = t0 > 0 ? 0 : 1;
-          if (!whole) pieces[place] = {t1 < s.tiles ? 1 : 2, s.q_begin + node0, h, nodes};
-          const int is = n_pub % kTrItems;
-          if (!t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) { ok = false; break; }
-          s_item[is] = {seq, h, s.q_begin + node0, node0, nodes, s.Lk - s.nodes, s.Lk, t0, n, split, whole ? -1 : 2 * static_cast<int>(blockIdx.x) + place};
-          mbar_arrive(&bar_item_full[is]);
-          ++n_pub;
-          // Q tiles: one, or two in turn
-          for (int x = 0; x < (split ? 1 : 2) && ok; ++x, ++q_use) {
-            const int b = q_use & 1;
-            if (!t2_wait_timed(&bar_q_empty[b], ((q_use >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
-            mbar_expect_tx(&bar_q_full[b], QT * G * 256);
-            tma_load_3d(sQ + b * kTrTile, &map_q, &bar_q_full[b], 0, h * G, s.q_begin + node0 + x * QT);
-            tma_load_3d(sQ + b * kTrTile + kTrSub, &map_q, &bar_q_full[b], 64, h * G, s.q_begin + node0 + x * QT);
-          }
-          if (!ok) break;
-          // K and V tiles in the order of their use: K runs ahead of V by the tiles that are in the halves
-          const int* const bt_row = p.block_tables + seq * p.bt_row_stride;
-          auto row_of = [&](int t) -> int {
-            const int key0 = (t0 + t) * kTrKv, col = key0 / p.block_size;
-            const long long blk = __ldg(bt_row + col);
-            return blk >= 0 && blk < p.num_blocks ? static_cast<int>(blk * p.block_size + (key0 - col * p.block_size)) : -(1 << 30);      // (nowhere: zeros)
-          };
-          auto load = [&](const CUtensorMap* map, const CUtensorMap* map16, int t) -> bool {
-            if (!t2_wait_timed(&bar_kv_empty[kv], kv_ph, abort_flag)) return false;
-            unsigned char* const dst = sKV + kv * kTrTile;
-            const int row0 = row_of(t), left = s.Lk - (t0 + t) * kTrKv;
-            if (left > kTrKv - 16) {
-              mbar_expect_tx(&bar_kv_full[kv], kTrTile);
-              tma_load_3d(dst, map, &bar_kv_full[kv], 0, h, row0);
-              tma_load_3d(dst + kTrSub, map, &bar_kv_full[kv], 64, h, row0);
-            } else {
-              // the sequence's last tile: only what it has of it
-              const int boxes = (left + 15) >> 4;
-              mbar_expect_tx(&bar_kv_full[kv], boxes * 4096);
-              for (int b = 0; b < boxes; ++b) {
-                tma_load_3d(dst + b * 2048, map16, &bar_kv_full[kv], 0, h, row0 + b * 16);
-                tma_load_3d(dst + kTrSub + b * 2048, map16, &bar_kv_full[kv], 64, h, row0 + b * 16);
-              }
+        const int t0 = from, t1 = !at_end ? s.tiles : unit == end_unit ? max(end_tile, from) : from;
+        const int block = unit / p.Hkv, h = unit - block * p.Hkv, node0 = block * 2 * QT, nodes = min(2 * QT, s.nodes - node0);
+        const int owner = seq;
+        ++unit;
+        from = 0;
+        if (at_end) seq = p.batch;
+        if (t0 == t1) continue;
+        const int split = nodes <= QT, q_row = s.q_begin + node0;
+        const bool whole = t0 == 0 && t1 == s.tiles;
+        const int place = t0 > 0 ? 0 : 1;
+        if (!whole) pieces[place] = {t1 < s.tiles ? 1 : 2, q_row, h, nodes};
+        const int is = n_pub % kTrItems;
+        if (!t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) { ok = false; break; }
+        s_item[is] = {owner, h, q_row, node0, nodes, s.Lk - s.nodes, s.Lk, t0, t1 - t0, split, turn, whole ? -1 : 2 * static_cast<int>(blockIdx.x) + place};
+        mbar_arrive(&bar_item_full[is]);
+        ++n_pub;
+        if (split) turn ^= (t1 - t0) & 1;
+        rows.start(p, owner, t0);
+        int row = rows.next(p), left = s.Lk - t0 * kTrKv;
+        if (!started) {
+          // everything so far overlaps the end of the kernel in front: lengths and tables, which it does not write
+          tma_prefetch_l2_3d(&map_k, 0, h, row);
+          tma_prefetch_l2_3d(&map_k, 64, h, row);
+          asm volatile("griddepcontrol.wait;" ::: "memory");
+          started = true;
+        }
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t) {
+          if (!t2_wait_timed(&bar_k_empty[k_at], k_ph, abort_flag)) { ok = false; break; }
+          tree_load(&map_k, &map_k16, &bar_k_full[k_at], sK + k_at * kTrTile, h, row, left);
+          if (++k_at == kTrRingK) { k_at = 0; k_ph ^= 1; }
+          if (t == t0) {
+            // its Q tile, or two
+#pragma unroll 1
+            for (int x = 0; x < (split ? 1 : 2); ++x, ++q_use) {
+              const int b = q_use & 1;
+              if (!t2_wait_timed(&bar_q_empty[b], ((q_use >> 1) & 1) ^ 1, abort_flag)) { ok = false; break; }
+              mbar_expect_tx(&bar_q_full[b], QT * G * 256);
+              tma_load_3d(sQ + b * kTrTile, &map_q, &bar_q_full[b], 0, h * G, q_row + x * QT);
+              tma_load_3d(sQ + b * kTrTile + kTrSub, &map_q, &bar_q_full[b], 64, h * G, q_row + x * QT);
             }
-            if (++kv == kTrRing) { kv = 0; kv_ph ^= 1; }
-            return true;
-          };
-          const int ahead = split ? 2 : 1;
-          for (int j = 0; j < ahead && j < n && ok; ++j) ok = load(&map_k, &map_k16, j);
-          for (int j = 0; j < n && ok; ++j) {
-            ok = load(&map_v, &map_v16, j);
-            if (ok && j + ahead < n) ok = load(&map_k, &map_k16, j + ahead);
+          }
+          if (t + 1 < t1) {
+            row = rows.next(p);
+            left -= kTrKv;
           }
         }
-        if (at_end) break;
-        ++unit;
-        t0 = 0;
       }
+      if (!started) asm volatile("griddepcontrol.wait;" ::: "memory");
       reinterpret_cast<int4*>(p.pieces)[2 * blockIdx.x] = make_int4(pieces[0].state, pieces[0].q_row, pieces[0].h, pieces[0].nodes);
       reinterpret_cast<int4*>(p.pieces)[2 * blockIdx.x + 1] = make_int4(pieces[1].state, pieces[1].q_row, pieces[1].h, pieces[1].nodes);
       if (ok) {
@@ -302,104 +359,101 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         }
       }
     } else if (warp == 1 && lane == 0) {
-      // ================================ MMA issuer ================================
+      // ================================ S = Q K^T ================================
       constexpr uint32_t idesc_qk = tc::idesc_bf16_f32(128, 128, false, false);
-      constexpr uint32_t idesc_pv = tc::idesc_bf16_f32(128, 128, false, true);
       constexpr uint32_t desc_hi = tc::smem_desc_sw128_hi(1024);
-      const uint32_t q_lo = tc::smem_desc_sw128_lo(smem_u32(sQ), 16), k_lo = tc::smem_desc_sw128_lo(smem_u32(sKV), 16);
-      const uint32_t v_lo = tc::smem_desc_sw128_lo(smem_u32(sKV), kTrSub);
-      int n_item = 0, kv = 0, kv_ph = 0, q_use = 0;
-      int np[2] = {0, 0}, no[2] = {0, 0};       // P tiles taken and accumulators finished per half
+      const uint32_t q_lo = tc::smem_desc_sw128_lo(smem_u32(sQ), 16), k_lo = tc::smem_desc_sw128_lo(smem_u32(sK), 16);
+      int n_item = 0, q_use = 0, k_at = 0, k_ph = 0, n_step = 0;
       bool ok = true;
-      auto next_kv = [&]() { if (++kv == kTrRing) { kv = 0; kv_ph ^= 1; } };
-      auto issue_s = [&](int hx, int q, int slot) {
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint32_t off = ((ks >> 2) * kTrSub + (ks & 3) * 32) >> 4;
-          tc::mma_ss_lo(tmem + hx * 128, q_lo + q * (kTrTile >> 4) + off, k_lo + slot * (kTrTile >> 4) + off, desc_hi, idesc_qk, ks > 0);
-        }
-        tc::commit(&bar_s_full[hx]);
-      };
-      auto issue_pv = [&](int hx, int slot, bool accumulate) {
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          tc::mma_ts_lo(tmem + 256 + hx * 128, tmem + hx * 128 + ks * 8, v_lo + slot * (kTrTile >> 4) + ks * (2048 >> 4), desc_hi, idesc_pv,
-                        accumulate || ks > 0);
-      };
       while (ok) {
         const int is = n_item % kTrItems;
         if (!t2_wait(&bar_item_full[is], (n_item / kTrItems) & 1, abort_flag)) break;
-        const int seq = s_item[is].seq, n = s_item[is].n;
-        const bool split = s_item[is].split;
+        const int seq = s_item[is].seq, split = s_item[is].split, steps = split ? s_item[is].n : 2 * s_item[is].n;
         mbar_arrive(&bar_item_empty[is]);
         if (seq < 0) break;
         ++n_item;
-        const int qa = q_use & 1, qb = split ? qa : qa ^ 1;
-        if (!t2_wait(&bar_q_full[qa], (q_use >> 1) & 1, abort_flag)) break;
-        ++q_use;
-        if (!split) {
-          if (!t2_wait(&bar_q_full[qb], (q_use >> 1) & 1, abort_flag)) break;
-          ++q_use;
-        }
-        // the first S of either half
-        if (!t2_wait_hot(&bar_kv_full[kv], kv_ph, abort_flag)) break;
-        tc::fence_after_sync();
-        issue_s(0, qa, kv);
-        if (split) {
-          tc::commit(&bar_kv_empty[kv]);
-          next_kv();
-          if (n > 1) {
-            if (!t2_wait_hot(&bar_kv_full[kv], kv_ph, abort_flag)) break;
-            tc::fence_after_sync();
-            issue_s(1, qa, kv);
-            tc::commit(&bar_kv_empty[kv]);
-            next_kv();
-          }
-          if (n <= 2) tc::commit(&bar_q_empty[qa]);
-        } else {
-          issue_s(1, qb, kv);
-          tc::commit(&bar_kv_empty[kv]);
-          next_kv();
-          if (n == 1) { tc::commit(&bar_q_empty[qa]); tc::commit(&bar_q_empty[qb]); }
-        }
-        // then P V of a tile, and the half's next S
-        const int ahead = split ? 2 : 1;
 #pragma unroll 1
-        for (int j = 0; j < n && ok; ++j) {
-          const int v_slot = kv;
-          if (!t2_wait_hot(&bar_kv_full[kv], kv_ph, abort_flag)) { ok = false; break; }
-          next_kv();
-          const bool more = j + ahead < n;
-          const int k_slot = kv;
-          if (more) {
-            if (!t2_wait_hot(&bar_kv_full[kv], kv_ph, abort_flag)) { ok = false; break; }
-            next_kv();
+        for (int at = 0; at < steps; ++at, ++n_step) {
+          const int hx = n_step & 1, second = !split && (at & 1);      // second: of the unit's two Q tiles
+          const int q = q_use + second;
+          if (at <= second && !t2_wait(&bar_q_full[q & 1], (q >> 1) & 1, abort_flag)) { ok = false; break; }
+          if (!t2_wait_hot(&bar_k_full[k_at], k_ph, abort_flag)) { ok = false; break; }
+          // (the scores of the step in front are in registers)
+          if (!t2_wait_hot(&bar_s_free, (n_step & 1) ^ 1, abort_flag)) { ok = false; break; }
+          tc::fence_after_sync();
+          const uint32_t d = tmem, qd = q_lo + (q & 1) * (kTrTile >> 4), kd = k_lo + k_at * (kTrTile >> 4);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint32_t off = ((ks >> 2) * kTrSub + (ks & 3) * 32) >> 4;
+            tc::mma_ss_lo(d, qd + off, kd + off, desc_hi, idesc_qk, ks > 0);
           }
-          const int h0 = split ? j & 1 : 0, h1 = split ? h0 : 1;
+          tc::commit(&bar_s_full[hx]);
+          if (split || second) {
+            tc::commit(&bar_k_empty[k_at]);
+            if (++k_at == kTrRingK) { k_at = 0; k_ph ^= 1; }
+          }
+          if (at + (split ? 1 : 2) >= steps) tc::commit(&bar_q_empty[q & 1]);
+        }
+        q_use += split ? 1 : 2;
+      }
+    } else if (warp == 2 && lane == 0) {
+      // ================================ O += P V ================================
+      // (A thread of its own: next to the softmax warps of its scheduler a single thread retires an instruction in 10 cycles, and
+      // what stands around the 16 products of a step took as long as they did.)
+      constexpr uint32_t idesc_pv = tc::idesc_bf16_f32(128, 128, false, true);
+      constexpr uint32_t desc_hi = tc::smem_desc_sw128_hi(1024);
+      const uint32_t v_lo = tc::smem_desc_sw128_lo(smem_u32(sV), kTrSub);
+      int n_item = 0, v_at = 0, v_ph = 0, n_step = 0, o_ph = 3;
+      bool ok = true;
+      while (ok) {
+        const int is = n_item % kTrItems;
+        if (!t2_wait(&bar_item_full[is], (n_item / kTrItems) & 1, abort_flag)) break;
+        const int seq = s_item[is].seq, split = s_item[is].split, steps = split ? s_item[is].n : 2 * s_item[is].n;
+        mbar_arrive(&bar_item_empty[is]);
+        if (seq < 0) break;
+        ++n_item;
 #pragma unroll 1
-          for (int hx = h0; hx <= h1; ++hx) {
-            // (the output warpgroup has taken the previous accumulator)
-            if (j < ahead && !t2_wait_hot(&bar_o_free[hx], (no[hx] & 1) ^ 1, abort_flag)) { ok = false; break; }
-            if (!t2_wait_hot(&bar_p_full[hx], np[hx] & 1, abort_flag)) { ok = false; break; }
-            ++np[hx];
-            tc::fence_after_sync();
-            issue_pv(hx, v_slot, j >= ahead);
-            if (more) {
-              issue_s(hx, hx && !split ? qb : qa, k_slot);
-            } else {
-              tc::commit(&bar_o_final[hx]);
-              ++no[hx];
-            }
+        for (int at = 0; at < steps; ++at, ++n_step) {
+          const int hx = n_step & 1;
+          if (!t2_wait_hot(&bar_v_full[v_at], v_ph, abort_flag)) { ok = false; break; }
+          if (at < 2) {
+            // the output warpgroup has taken the accumulator of the unit in front
+            if (!t2_wait_hot(&bar_o_free[hx], (o_ph >> hx) & 1, abort_flag)) { ok = false; break; }
+            o_ph ^= 1 << hx;
           }
-          if (!ok) break;
-          tc::commit(&bar_kv_empty[v_slot]);
-          if (more) {
-            tc::commit(&bar_kv_empty[k_slot]);
-            if (j + ahead + 1 == n) {       // the unit's last S
-              tc::commit(&bar_q_empty[qa]);
-              if (!split) tc::commit(&bar_q_empty[qb]);
-            }
+          if (!t2_wait_hot(&bar_p_full[hx], (n_step >> 1) & 1, abort_flag)) { ok = false; break; }
+          tc::fence_after_sync();
+          const uint32_t d = tmem + 256 + hx * 128, a = tmem + 128 + hx * 64, v = v_lo + v_at * (kTrTile >> 4);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) tc::mma_ts_lo(d, a + ks * 8, v + ks * (2048 >> 4), desc_hi, idesc_pv, at >= 2 || ks > 0);
+          tc::commit(&bar_pv[hx]);
+          if (at + 2 >= steps) tc::commit(&bar_o_final[hx]);
+          if (split || (at & 1)) {
+            tc::commit(&bar_v_empty[v_at]);
+            if (++v_at == kTrRingV) { v_at = 0; v_ph ^= 1; }
           }
+        }
+      }
+    } else if (warp == 3 && lane == 0) {
+      // ================================ V ================================
+      TreeRows rows = {};
+      int n_item = 0, v_at = 0, v_ph = 1;
+      bool ok = true;
+      while (ok) {
+        const int is = n_item % kTrItems;
+        if (!t2_wait(&bar_item_full[is], (n_item / kTrItems) & 1, abort_flag)) break;
+        const int seq = s_item[is].seq, h = s_item[is].h, t0 = s_item[is].t0, n = s_item[is].n;
+        int left = s_item[is].Lk - t0 * kTrKv;
+        mbar_arrive(&bar_item_empty[is]);
+        if (seq < 0) break;
+        ++n_item;
+        rows.start(p, seq, t0);
+#pragma unroll 1
+        for (int j = 0; j < n; ++j, left -= kTrKv) {
+          const int row = rows.next(p);
+          if (!t2_wait(&bar_v_empty[v_at], v_ph, abort_flag)) { ok = false; break; }
+          tree_load(&map_v, &map_v16, &bar_v_full[v_at], sV + v_at * kTrTile, h, row, left);
+          if (++v_at == kTrRingV) { v_at = 0; v_ph ^= 1; }
         }
       }
     }
@@ -409,10 +463,11 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     const int hx = (warp - 4) >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;                  // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t tmem_s = tmem + hx * 128 + lane_base, tmem_o = tmem + 256 + hx * 128 + lane_base;
+    const uint32_t tmem_s = tmem + lane_base, tmem_p = tmem + 128 + hx * 64 + lane_base, tmem_o = tmem + 256 + hx * 128 + lane_base;
     const float c = p.scale_log2;
     int n_item = 0, ns = 0, n_fin = 0;
-    int kv = 0, kv_ph = 0;                              // the ring's place behind the unit
+    int v_at = 0, v_ph = 0;                             // place and phase in the V ring of the unit's last tile
+    int v_next = 0;                                     // (tiles so far, modulo the ring's two turns)
     bool ok = true;
     while (ok) {
       const int is = n_item % kTrItems;
@@ -422,67 +477,67 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       if (lane == 0) mbar_arrive(&bar_item_empty[is]);
       if (it.seq < 0) break;
       ++n_item;
-      const int nx = it.split ? (hx ? it.n >> 1 : (it.n + 1) >> 1) : it.n;
-      const int tile_nodes = it.split || !hx ? min(it.nodes, QT) : it.nodes - QT;
+      const int mine = hx ^ it.turn;                             // 0: this half takes the unit's first step
+      const int nx = it.split ? (it.n + 1 - mine) >> 1 : it.n;
+      const int tile = it.split ? 0 : mine;                      // the Q tile
+      const int tile_nodes = tile ? it.nodes - QT : min(it.nodes, QT);
       const bool active = quarter * 32 < tile_nodes * G;         // this warp has rows
-      const int in_tile = r / G + (it.split || !hx ? 0 : QT);    // the row's node within the unit
+      const int in_tile = r / G + tile * QT;                     // the row's node within the unit
       const bool row_ok = in_tile < it.nodes && r < QT * G;
-      const uint32_t* const mask = p.masks && row_ok ? p.masks + static_cast<long long>(it.q_row + in_tile) * p.mask_words : nullptr;
-      // (rows that are none see nothing: a chain's row of index -1 - nodes)
-      const int node = row_ok ? it.node0 + in_tile : -0x40000000;
       const bool chain = p.masks == nullptr;
-      // place of the unit's last V tile in the ring, for its ragged tile
-      int last_kv = kv + 2 * it.n - 1;
-      int last_ph = kv_ph;
-      { const int turns = last_kv / kTrRing; last_kv -= turns * kTrRing; last_ph ^= turns & 1; }
-      { const int behind = kv + 2 * it.n, turns = behind / kTrRing; kv = behind - turns * kTrRing; kv_ph ^= turns & 1; }
+      const uint32_t* const mask = !chain && row_ok ? p.masks + static_cast<long long>(it.q_row + in_tile) * p.mask_words : nullptr;
+      if (mask && (it.t0 + it.n) * kTrKv > it.first) asm volatile("prefetch.global.L1 [%0];" ::"l"(mask));
+      // (rows that are none see nothing: a chain's row of an index below all)
+      const int node = row_ok ? it.node0 + in_tile : -0x40000000;
+      v_next = (v_next + it.n) % (2 * kTrRingV);
+      { const int last = v_next ? v_next - 1 : 2 * kTrRingV - 1; v_at = last % kTrRingV; v_ph = last / kTrRingV; }
       float m_used = -INFINITY, l = 0.f;
       for (int j = 0; j < nx; ++j) {
         if (!t2_wait_hot(&bar_s_full[hx], ns & 1, abort_flag)) { ok = false; break; }
         ++ns;
-        const int key0 = (it.t0 + (it.split ? 2 * j + hx : j)) * kTrKv;
+        const int key0 = (it.t0 + (it.split ? 2 * j + mine : j)) * kTrKv;
         if (active) {
           tc::fence_after_sync();
+          if (key0 + kTrKv > min(it.first, it.Lk)) {
+            // the tile reaches the nodes: masked scores go back over S first (rolled: the hot code stays short)
+#pragma unroll 1
+            for (int cch = 0; cch < 4; ++cch) {
+              const int col = key0 + cch * 32;
+              const uint32_t keep = chain || row_ok ? tree_keep32(mask, p.mask_words, node, col - it.first, it.Lk - col) : 0u;
+              if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
+              uint32_t v[32];
+              tc::ld_32x32b_x32(tmem_s + cch * 32, v);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!((keep >> i) & 1)) v[i] = 0xff800000u;   // -inf
+              tc::st_32x32b_x32(tmem_s + cch * 32, v);
+            }
+            tc::wait_st();
+          }
+          // the whole S row in registers: four TMEM loads in flight, one wait; eight independent chains of 3-input max
           uint32_t sv[4][32];
 #pragma unroll
           for (int cch = 0; cch < 4; ++cch) tc::ld_32x32b_x32(tmem_s + cch * 32, sv[cch]);
           tc::wait_ld();
-          if (key0 + kTrKv > min(it.first, it.Lk)) {
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar_s_free);
+          float m8[8] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int cch = 0; cch < 4; ++cch) {
-              const int d = key0 + cch * 32 - it.first, left = it.Lk - key0 - cch * 32;
-              const uint32_t keep = chain || row_ok ? tree_keep32(chain ? nullptr : mask, p.mask_words, node, d, left) : 0u;
-              if (keep != 0xffffffffu) {
+          for (int cch = 0; cch < 4; ++cch)
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (!((keep >> i) & 1)) sv[cch][i] = 0xff800000u;   // -inf
-              }
-            }
-          }
-          // eight independent chains of 3-input max
-          float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
-          float mx4 = -INFINITY, mx5 = -INFINITY, mx6 = -INFINITY, mx7 = -INFINITY;
-#pragma unroll
-          for (int cch = 0; cch < 4; ++cch) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 16) {
-              mx0 = fmax3(mx0, __uint_as_float(sv[cch][i]), __uint_as_float(sv[cch][i + 1]));
-              mx1 = fmax3(mx1, __uint_as_float(sv[cch][i + 2]), __uint_as_float(sv[cch][i + 3]));
-              mx2 = fmax3(mx2, __uint_as_float(sv[cch][i + 4]), __uint_as_float(sv[cch][i + 5]));
-              mx3 = fmax3(mx3, __uint_as_float(sv[cch][i + 6]), __uint_as_float(sv[cch][i + 7]));
-              mx4 = fmax3(mx4, __uint_as_float(sv[cch][i + 8]), __uint_as_float(sv[cch][i + 9]));
-              mx5 = fmax3(mx5, __uint_as_float(sv[cch][i + 10]), __uint_as_float(sv[cch][i + 11]));
-              mx6 = fmax3(mx6, __uint_as_float(sv[cch][i + 12]), __uint_as_float(sv[cch][i + 13]));
-              mx7 = fmax3(mx7, __uint_as_float(sv[cch][i + 14]), __uint_as_float(sv[cch][i + 15]));
-            }
-          }
-          const float mx = fmax3(fmax3(mx0, mx1, mx2), fmax3(mx3, mx4, mx5), fmaxf(mx6, mx7));
+            for (int i = 0; i < 32; i += 2)
+              m8[(i >> 1) & 7] = fmax3(m8[(i >> 1) & 7], __uint_as_float(sv[cch][i]), __uint_as_float(sv[cch][i + 1]));
+          const float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
           const float m_new = fmaxf(m_used, mx);
           if (j == 0) {
             m_used = m_new;
           } else {
             const bool grow = (m_new - m_used) * c > kTrRescale;
             if (__any_sync(0xffffffffu, grow)) {
+              if (!t2_wait_hot(&bar_pv[hx], ns & 1, abort_flag)) { ok = false; break; }
+              tc::fence_after_sync();
               const float alpha = grow ? fast_exp2((m_used - m_new) * c) : 1.f;
               if (grow) { m_used = m_new; l *= alpha; }
 #pragma unroll 1
@@ -521,18 +576,29 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
               pk[i + 2] = pack_bf16(p4, p5);
               pk[i + 3] = pack_bf16(p6, p7);
             }
-            tc::st_32x32b_x16(tmem_s + cch * 16, pk);
+            if (cch == 0 && ns > 1) {
+              // the P of the half's step in front has been used
+              if (!t2_wait_hot(&bar_pv[hx], ns & 1, abort_flag)) { ok = false; break; }
+              tc::fence_after_sync();
+            }
+            tc::st_32x32b_x16(tmem_p + cch * 16, pk);
           }
+          if (!ok) break;
           float a0, a1;
           f32x2_unpack(f32x2_add(f32x2_add(ls0, ls1), f32x2_add(ls2, ls3)), a0, a1);
           l += a0 + a1;
           tc::wait_st();
+        } else {
+          if (lane == 0) mbar_arrive(&bar_s_free);
+          // (no rows, but in step with the others: the next S comes ahead of this one's P V, and its arrival below must not count
+          // for the step in front)
+          if (ns > 1 && !t2_wait(&bar_pv[hx], ns & 1, abort_flag)) { ok = false; break; }
         }
         if (key0 + kTrKv > it.Lk) {
           // The sequence's last tile: V rows behind its end are stale or foreign; zero them, so that 0 * garbage cannot turn into
           // NaN in the tensor core.  (It is the unit's last V tile.)
-          if (!t2_wait_hot(&bar_kv_full[last_kv], last_ph, abort_flag)) { ok = false; break; }
-          unsigned char* const rows = sKV + last_kv * kTrTile;
+          if (!t2_wait_hot(&bar_v_full[v_at], v_ph, abort_flag)) { ok = false; break; }
+          unsigned char* const rows = sV + v_at * kTrTile;
 #pragma unroll 1
           for (int i = (it.Lk - key0) * 128 + r * 16; i < kTrSub; i += 128 * 16) {
             *reinterpret_cast<uint4*>(rows + i) = make_uint4(0, 0, 0, 0);
@@ -575,11 +641,12 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
 #pragma unroll 1
       for (int turn = 0; turn < (it.split ? 1 : 2) && ok; ++turn) {
         const bool joined = it.split && it.n > 1;
+        const int h0 = it.turn ^ turn;                   // the half that has it; joined: the other, too
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (e == 1 && !joined) continue;
-          const int hx = turn + e;
+          const int hx = h0 ^ e;
           if (!t2_wait(&bar_l_full[hx], nf[hx] & 1, abort_flag)) { ok = false; break; }
           m[e] = s_max[hx][r];
           l[e] = s_sum[hx][r];
@@ -607,22 +674,21 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
             wa *= inv;
             wb *= inv;
           }
-          const uint32_t ta = tmem + 256 + turn * 128 + lane_base;
+          const uint32_t ta = tmem + 256 + h0 * 128 + lane_base, tb = tmem + 384 - h0 * 128 + lane_base;
 #pragma unroll 1
           for (int cch = 0; cch < 8; ++cch) {
             uint32_t a[16];
             tc::ld_32x32b_x16(ta + cch * 16, a);
+            uint32_t b[16];
             if (joined) {
-              uint32_t b[16];
-              tc::ld_32x32b_x16(ta + 128 + cch * 16, b);
-              tc::wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), wb, __uint_as_float(a[i]) * wa));
+              tc::ld_32x32b_x16(tb + cch * 16, b);
             } else {
-              tc::wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * wa);
+              for (int i = 0; i < 16; ++i) b[i] = 0;
             }
+            tc::wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), wb, __uint_as_float(a[i]) * wa));
             if (part) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) part[(cch * 16 + i) * 32] = __uint_as_float(a[i]);
@@ -642,8 +708,8 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         tc::fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&bar_o_free[turn]);
-          if (joined) mbar_arrive(&bar_o_free[1]);
+          mbar_arrive(&bar_o_free[h0]);
+          if (joined) mbar_arrive(&bar_o_free[h0 ^ 1]);
         }
       }
     }
@@ -652,7 +718,6 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   // ---- teardown: everyone meets, then the allocating warp frees TMEM ----
   tc::fence_before_sync();
   __syncthreads();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp == 1) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, 512);
@@ -660,47 +725,149 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   if (tid == 0 && s_abort) atomicExch(&g_status_tree, 1);
 }
 
-// Units that a cut ran through: a CTA per (cut, group of 32 rows), the cut that is a unit's first joins all of its pieces, in their
-// order.  A warp takes 8 of the 128 dims, a lane a row.
-constexpr int kTrJoinThreads = 512;
-__global__ void __launch_bounds__(kTrJoinThreads)
-tree_join_kernel(const TreeParams p, int ctas) {
+// Units that a cut ran through.  Every CTA reads all records and lists the pieces in their order (a unit's first and last ones
+// alternate in it).  A task is (unit, group of 32 rows, some of the dims: the more pieces, the fewer, so that a task's partial
+// results fit the buffer); they come as bulk copies, all under way at once, because what takes time here is the round trip to L2.
+// The code is short for the same reason: it is fetched anew for every launch.
+constexpr int kTrJoinThreads = 128;
+constexpr int kTrJoinCtas = 5;                // per SM
+constexpr int kTrMaxCtas = 160;               // of the kernel above (a B200 has 148 multiprocessors)
+constexpr int kTrJoinPieces = 16;
+constexpr int kTrJoinFloats = kTrJoinPieces * (16 * 32 + 64);
+
+struct JoinShared {
+  __align__(128) float buf[kTrJoinFloats];
+  float weight[kTrJoinPieces][32];
+  int4 piece[2 * kTrMaxCtas];                 // TreePiece
+  int task[kTrMaxCtas + 1];                   // first task of a unit
+  short list[2 * kTrMaxCtas], first[kTrMaxCtas], last[kTrMaxCtas];
+  uint64_t bar;
+  int units, abort;
+};
+static_assert(sizeof(JoinShared) <= 48 * 1024, "static shared memory");
+// Slices of the 128 dims that a unit of n pieces is cut into, as a shift.
+__device__ __forceinline__ int join_shift(int n) { return n <= 2 ? 0 : n <= 4 ? 1 : n <= 8 ? 2 : 3; }
+
+__global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreeParams p, int ctas) {
+  __shared__ JoinShared s;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.G, QT = 128 / G;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    s.abort = 0;
+    mbar_init(&s.bar, 1);
+    mbar_fence_init();
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int cut = blockIdx.x + 1, group = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int4* const pieces = reinterpret_cast<const int4*>(p.pieces);
-  const int4 head = __ldcg(pieces + 2 * (cut - 1) + 1);
-  if (head.x != 1) return;
-  const int G = p.G, QT = 128 / G, half = group >> 2, r = (group & 3) * 32 + lane;
-  const int nodes = min(head.w - half * QT, QT);      // of this half
-  if ((group & 3) * 32 >= nodes * G) return;
-  const float* const mine = p.partials + static_cast<long long>(group) * kTrGroup + lane;
-  auto part = [&](int place) { return mine + static_cast<long long>(place) * kTrPartial; };
-  // the pieces: the first one's place, then the next CTAs' first places until the last
-  float M = ld_cg_f32(part(2 * (cut - 1) + 1) + 128 * 32);
-  int last = cut;
-  for (;; ++last) {
-    const int state = __ldcg(pieces + 2 * last).x;
-    if (state) M = fmaxf(M, ld_cg_f32(part(2 * last) + 128 * 32));
-    if (state == 2 || last + 1 >= ctas) break;
-  }
-  float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int c = cut - 1; c <= last; ++c) {
-    if (c >= cut && !__ldcg(pieces + 2 * c).x) continue;
-    const float* const from = part(c < cut ? 2 * c + 1 : 2 * c);
-    const float w = M == -INFINITY ? 0.f : fast_exp2(ld_cg_f32(from + 128 * 32) - M);
-    sum = fmaf(ld_cg_f32(from + 129 * 32), w, sum);
+#pragma unroll 3
+  for (int e = tid; e < 2 * ctas; e += kTrJoinThreads) s.piece[e] = __ldcg(reinterpret_cast<const int4*>(p.pieces) + e);
+  __syncthreads();
+  if (warp == 0) {
+    const unsigned below = (1u << lane) - 1;
+    int pieces = 0, firsts = 0, lasts = 0;
+#pragma unroll 1
+    for (int e = lane; e - lane < 2 * ctas; e += 32) {
+      const int state = e < 2 * ctas ? s.piece[e].x : 0;
+      const bool is_first = state && (e & 1), is_last = state == 2;
+      const unsigned any = __ballot_sync(0xffffffffu, state != 0), first = __ballot_sync(0xffffffffu, is_first), last = __ballot_sync(0xffffffffu, is_last);
+      const int at = pieces + __popc(any & below);
+      if (state) s.list[at] = static_cast<short>(e);
+      if (is_first) s.first[firsts + __popc(first & below)] = static_cast<short>(at);
+      if (is_last) s.last[lasts + __popc(last & below)] = static_cast<short>(at);
+      pieces += __popc(any);
+      firsts += __popc(first);
+      lasts += __popc(last);
+    }
+    __syncwarp();
+    const int units = min(firsts, lasts);          // (equal, unless the kernel in front gave up)
+    int before = 0;
+#pragma unroll 1
+    for (int u = lane; u - lane < units; u += 32) {
+      int x = 0;
+      if (u < units) {
+        const int a = s.first[u], nodes = s.piece[s.list[a]].w;
+        const int groups = (min(nodes, QT) * G + 31) / 32 + (max(nodes - QT, 0) * G + 31) / 32;
+        x = groups << join_shift(s.last[u] - a + 1);
+      }
+      const int mine = x;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = fmaf(ld_cg_f32(from + (warp * 8 + i) * 32), w, o[i]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (u < units) s.task[u] = before + x - mine;
+      before += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) {
+      s.units = units;
+      s.task[units] = before;
+    }
   }
-  if (r >= nodes * G) return;
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  const int t = r / G;
-  uint4 v;
-  v.x = pack_bf16(o[0] * inv, o[1] * inv);
-  v.y = pack_bf16(o[2] * inv, o[3] * inv);
-  v.z = pack_bf16(o[4] * inv, o[5] * inv);
-  v.w = pack_bf16(o[6] * inv, o[7] * inv);
-  reinterpret_cast<uint4*>(p.out + (static_cast<long long>(head.y + half * QT + t) * p.H + head.z * G + (r - t * G)) * 128)[warp] = v;
+  __syncthreads();
+  const int units = s.units, tasks = s.task[units];
+  int loads = 0;                                   // phases of the barrier
+#pragma unroll 1
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    int u = 0, hi = units;
+    while (hi - u > 1) {
+      const int mid = (u + hi) >> 1;
+      if (s.task[mid] <= task) u = mid; else hi = mid;
+    }
+    const int a = s.first[u], n = s.last[u] - a + 1, shift = join_shift(n), dims = 128 >> shift;
+    const int4 head = s.piece[s.list[a]];
+    const int at = task - s.task[u], dim0 = (at & ((1 << shift) - 1)) * dims, groups0 = (min(head.w, QT) * G + 31) / 32;
+    const int half = (at >> shift) >= groups0, group = half ? 4 + (at >> shift) - groups0 : at >> shift;
+    const int r = (group & 3) * 32 + lane, nodes = half ? head.w - QT : min(head.w, QT), t = r / G;
+    __nv_bfloat16* const dst = p.out + (static_cast<long long>(head.y + half * QT + t) * p.H + head.z * G + (r - t * G)) * 128 + dim0;
+    const int stride = dims * 32 + 64;             // floats of a piece in the buffer: its dims, then maxima and sums
+    float M = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int base = 0; base < n; base += kTrJoinPieces) {
+      const int m = min(n - base, kTrJoinPieces);
+      __syncthreads();                             // the buffer has been read
+      if (tid == 0) mbar_expect_tx(&s.bar, m * stride * 4);
+      __syncwarp();
+      if (tid < m) {
+        const float* const from = p.partials + s.list[a + base + tid] * static_cast<long long>(kTrPartial) + group * kTrGroup;
+        tree_bulk_load(s.buf + tid * stride, from + dim0 * 32, dims * 128, &s.bar);
+        tree_bulk_load(s.buf + tid * stride + dims * 32, from + 128 * 32, 256, &s.bar);
+      }
+      if (!mbar_wait(&s.bar, loads & 1, &s.abort)) {
+        if (tid == 0) atomicExch(&g_status_tree, 1);
+        return;
+      }
+      ++loads;
+      // every warp for itself: the new maximum and sum; the weights are shared out
+      float top = M;
+#pragma unroll 4
+      for (int x = 0; x < m; ++x) top = fmaxf(top, s.buf[x * stride + dims * 32 + lane]);
+      const float ref = top == -INFINITY ? 0.f : top, was = fast_exp2(M - ref);
+      M = top;
+      sum *= was;
+#pragma unroll 4
+      for (int x = 0; x < m; ++x) {
+        const float w = fast_exp2(s.buf[x * stride + dims * 32 + lane] - ref);
+        sum = fmaf(s.buf[x * stride + dims * 32 + 32 + lane], w, sum);
+        if ((x & 3) == warp) s.weight[x][lane] = w;
+      }
+      __syncthreads();
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      // 4 dims of a warp at a time (with 16 dims in all, once: more pieces may follow)
+#pragma unroll 1
+      for (int d = warp * 4; d < dims; d += 16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = base ? o[i] * was : 0.f;
+#pragma unroll 2
+        for (int x = 0; x < m; ++x) {
+          const float w = s.weight[x][lane];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = fmaf(s.buf[x * stride + (d + i) * 32 + lane], w, o[i]);
+        }
+        if (base + m == n && r < nodes * G)
+          *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+      }
+    }
+  }
 }
 
 // Workspace: the pieces' records, then two places of partial results per CTA.
@@ -775,7 +942,12 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.Hkv = num_kv_heads;
   p.G = G;
   p.scale_log2 = scale * 1.4426950408889634f;
+  // the longest that the line of key tiles can be (table widths are all that the host knows of the lengths)
+  const double line = static_cast<double>(num_kv_heads) * (total_q / (2 * (128 / G)) + batch) *
+                      (static_cast<double>(bt_cols) * (block_size / kTrKv) * kTrCostPair + kTrCostUnit);
+  if (line >= 2147483648.0) return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
   const int grid = sm_count();
+  if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
   p.pieces = static_cast<int*>(workspace);
   p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_pieces_bytes(grid));
   CUtensorMap map_q, map_k, map_v, map_k16, map_v16;
@@ -786,7 +958,7 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   if (!rc) rc = make_tokens_heads_map(&map_k16, k_cache, rows, num_kv_heads, row, 16);
   if (!rc) rc = make_tokens_heads_map(&map_v16, v_cache, rows, num_kv_heads, row, 16);
   if (rc) return rc;
-  const size_t smem = static_cast<size_t>(2 + kTrRing) * kTrTile;
+  const size_t smem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTile;
   static std::atomic<size_t> configured[kMaxDevices];
   rc = ensure_dynamic_smem(reinterpret_cast<const void*>(tree_attn_kernel), smem, configured, "tree_attn: cudaFuncSetAttribute");
   if (rc) return rc;
@@ -794,18 +966,7 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   g_launches.fetch_add(1);
   rc = check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn launch");
   if (rc || grid < 2) return rc;
-  // rows of the largest unit there can be, in groups of 32; a unit of two tiles has its second tile's rows from group 4 on
-  const long long most = total_q <= 128 / G ? (static_cast<long long>(total_q) * G + 31) / 32 : 8;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid - 1, static_cast<unsigned>(most));
-  cfg.blockDim = dim3(kTrJoinThreads);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  le = cudaLaunchKernelEx(&cfg, tree_join_kernel, p, grid);
+  le = launch_early(tree_join_kernel, grid * kTrJoinCtas, kTrJoinThreads, 0, static_cast<cudaStream_t>(stream), p, grid);
   g_launches.fetch_add(1);
   return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn join launch");
 }
