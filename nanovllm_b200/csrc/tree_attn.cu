@@ -65,10 +65,13 @@ __device__ __forceinline__ void tree_bulk_load(void* dst, const void* src, uint3
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-// What a cut unit's pieces are: a record for each place of partial results, written by every CTA.
-struct TreePiece {
-  int state;            // 0: none, 1: more of the unit follows, 2: its last
-  int q_row, h, nodes;
+// What a cut unit's pieces are, for the join.  A CTA's share can begin within a unit (its partial results go to place 2 * CTA) and end
+// within one that it began (place 2 * CTA + 1).  Every CTA writes its entries.
+constexpr int kTrMaxCtas = 160;               // (a B200 has 148 multiprocessors)
+struct TreePieces {
+  int head[kTrMaxCtas];                       // nodes of the unit that the share ends within, 0: none
+  int cont[kTrMaxCtas];                       // the share begins within a unit: 1, or 2 if it has the unit's last tile, too; 0: it does not
+  int2 unit[kTrMaxCtas];                      // where head is set: the unit's first row, its kv head
 };
 
 // One sequence as the line sees it.
@@ -279,7 +282,8 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       tma_prefetch_desc(&map_q);
       tma_prefetch_desc(&map_k);
       tma_prefetch_desc(&map_v);
-      TreePiece pieces[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+      int cont = 0, head = 0;
+      int2 head_unit = make_int2(0, 0);
       int seq = s_at[0][0], unit = s_at[0][1], from = s_at[0][2], have = -1;
       TreeSeq s = {};
       TreeRows rows = {};
@@ -309,7 +313,12 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         const int split = nodes <= QT, q_row = s.q_begin + node0;
         const bool whole = t0 == 0 && t1 == s.tiles;
         const int place = t0 > 0 ? 0 : 1;
-        if (!whole) pieces[place] = {t1 < s.tiles ? 1 : 2, q_row, h, nodes};
+        if (t0 > 0) {
+          cont = t1 < s.tiles ? 1 : 2;
+        } else if (!whole) {
+          head = nodes;
+          head_unit = make_int2(q_row, h);
+        }
         const int is = n_pub % kTrItems;
         if (!t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) { ok = false; break; }
         s_item[is] = {owner, h, q_row, node0, nodes, s.Lk - s.nodes, s.Lk, t0, t1 - t0, split, turn, whole ? -1 : 2 * static_cast<int>(blockIdx.x) + place};
@@ -348,8 +357,9 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         }
       }
       if (!started) asm volatile("griddepcontrol.wait;" ::: "memory");
-      reinterpret_cast<int4*>(p.pieces)[2 * blockIdx.x] = make_int4(pieces[0].state, pieces[0].q_row, pieces[0].h, pieces[0].nodes);
-      reinterpret_cast<int4*>(p.pieces)[2 * blockIdx.x + 1] = make_int4(pieces[1].state, pieces[1].q_row, pieces[1].h, pieces[1].nodes);
+      p.pieces->cont[blockIdx.x] = cont;
+      p.pieces->head[blockIdx.x] = head;
+      p.pieces->unit[blockIdx.x] = head_unit;
       if (ok) {
         const int is = n_pub % kTrItems;
         if (t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) {
@@ -725,154 +735,147 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   if (tid == 0 && s_abort) atomicExch(&g_status_tree, 1);
 }
 
-// Units that a cut ran through.  Every CTA reads all records and lists the pieces in their order (a unit's first and last ones
-// alternate in it).  A task is (unit, group of 32 rows, some of the dims: the more pieces, the fewer, so that a task's partial
-// results fit the buffer); they come as bulk copies, all under way at once, because what takes time here is the round trip to L2.
-// The code is short for the same reason: it is fetched anew for every launch.
+// Units that a cut ran through.  A task is (unit, group of 32 rows, some of the dims: the fewer units, the fewer); its partial results
+// come as bulk copies, all under way at once.  What takes time here is round trips to L2 and fetching the code, which is new
+// for every launch: so every warp reads all records (five words a lane) and finds its unit and pieces by bits of ballots.
 constexpr int kTrJoinThreads = 128;
 constexpr int kTrJoinCtas = 5;                // per SM
-constexpr int kTrMaxCtas = 160;               // of the kernel above (a B200 has 148 multiprocessors)
-constexpr int kTrJoinPieces = 16;
+constexpr int kTrJoinPieces = 16;             // of 16 dims; 2 of 128
 constexpr int kTrJoinFloats = kTrJoinPieces * (16 * 32 + 64);
-
-struct JoinShared {
-  __align__(128) float buf[kTrJoinFloats];
-  float weight[kTrJoinPieces][32];
-  int4 piece[2 * kTrMaxCtas];                 // TreePiece
-  int task[kTrMaxCtas + 1];                   // first task of a unit
-  short list[2 * kTrMaxCtas], first[kTrMaxCtas], last[kTrMaxCtas];
-  uint64_t bar;
-  int units, abort;
-};
-static_assert(sizeof(JoinShared) <= 48 * 1024, "static shared memory");
-// Slices of the 128 dims that a unit of n pieces is cut into, as a shift.
-__device__ __forceinline__ int join_shift(int n) { return n <= 2 ? 0 : n <= 4 ? 1 : n <= 8 ? 2 : 3; }
+constexpr int kTrJoinWords = kTrMaxCtas / 32;
 
 __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreeParams p, int ctas) {
-  __shared__ JoinShared s;
+  __shared__ __align__(128) float s_buf[kTrJoinFloats];
+  __shared__ float s_weight[kTrJoinPieces][32];
+  __shared__ short s_list[kTrMaxCtas + 1];    // places of the unit's pieces
+  __shared__ __align__(8) uint64_t s_bar;
+  __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.G, QT = 128 / G;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
-    s.abort = 0;
-    mbar_init(&s.bar, 1);
+    s_abort = 0;
+    mbar_init(&s_bar, 1);
     mbar_fence_init();
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-#pragma unroll 3
-  for (int e = tid; e < 2 * ctas; e += kTrJoinThreads) s.piece[e] = __ldcg(reinterpret_cast<const int4*>(p.pieces) + e);
-  __syncthreads();
-  if (warp == 0) {
-    const unsigned below = (1u << lane) - 1;
-    int pieces = 0, firsts = 0, lasts = 0;
-#pragma unroll 1
-    for (int e = lane; e - lane < 2 * ctas; e += 32) {
-      const int state = e < 2 * ctas ? s.piece[e].x : 0;
-      const bool is_first = state && (e & 1), is_last = state == 2;
-      const unsigned any = __ballot_sync(0xffffffffu, state != 0), first = __ballot_sync(0xffffffffu, is_first), last = __ballot_sync(0xffffffffu, is_last);
-      const int at = pieces + __popc(any & below);
-      if (state) s.list[at] = static_cast<short>(e);
-      if (is_first) s.first[firsts + __popc(first & below)] = static_cast<short>(at);
-      if (is_last) s.last[lasts + __popc(last & below)] = static_cast<short>(at);
-      pieces += __popc(any);
-      firsts += __popc(first);
-      lasts += __popc(last);
-    }
-    __syncwarp();
-    const int units = min(firsts, lasts);          // (equal, unless the kernel in front gave up)
-    int before = 0;
-#pragma unroll 1
-    for (int u = lane; u - lane < units; u += 32) {
-      int x = 0;
-      if (u < units) {
-        const int a = s.first[u], nodes = s.piece[s.list[a]].w;
-        const int groups = (min(nodes, QT) * G + 31) / 32 + (max(nodes - QT, 0) * G + 31) / 32;
-        x = groups << join_shift(s.last[u] - a + 1);
-      }
-      const int mine = x;
+  int head[kTrJoinWords], cont[kTrJoinWords];
+  int2 unit_of[kTrJoinWords];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (u < units) s.task[u] = before + x - mine;
-      before += __shfl_sync(0xffffffffu, x, 31);
-    }
-    if (lane == 0) {
-      s.units = units;
-      s.task[units] = before;
-    }
+  for (int w = 0; w < kTrJoinWords; ++w) {
+    const int c = w * 32 + lane;
+    head[w] = c < ctas ? __ldcg(p.pieces->head + c) : 0;
+    cont[w] = c < ctas ? __ldcg(p.pieces->cont + c) : 0;
+    unit_of[w] = c < ctas ? __ldcg(p.pieces->unit + c) : make_int2(0, 0);
   }
-  __syncthreads();
-  const int units = s.units, tasks = s.task[units];
-  int loads = 0;                                   // phases of the barrier
+  unsigned heads[kTrJoinWords];
+  int units = 0;
+#pragma unroll
+  for (int w = 0; w < kTrJoinWords; ++w) {
+    heads[w] = __ballot_sync(0xffffffffu, head[w] > 0);
+    units += __popc(heads[w]);
+  }
+  // tasks of a unit: 8 groups x 1, 2, 4 or 8 slices of the dims, so that there are about as many as CTAs
+  const int shift = units > 74 ? 0 : units > 37 ? 1 : units > 18 ? 2 : 3;
+  int loads = 0;                              // phases of the barrier
 #pragma unroll 1
-  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
-    int u = 0, hi = units;
-    while (hi - u > 1) {
-      const int mid = (u + hi) >> 1;
-      if (s.task[mid] <= task) u = mid; else hi = mid;
+  for (int task = blockIdx.x; task < units << (3 + shift); task += gridDim.x) {
+    // the unit: the CTA that has its first piece, and how many nodes
+    int k = task >> (3 + shift), c0 = 0, nodes_all = 0;
+    int2 unit = make_int2(0, 0);
+#pragma unroll
+    for (int w = 0; w < kTrJoinWords; ++w) {
+      const unsigned found = __ballot_sync(0xffffffffu, head[w] > 0 && __popc(heads[w] & ((1u << lane) - 1)) == k);
+      if (found) {
+        c0 = w * 32 + __ffs(found) - 1;
+        nodes_all = __shfl_sync(0xffffffffu, head[w], __ffs(found) - 1);
+        unit.x = __shfl_sync(0xffffffffu, unit_of[w].x, __ffs(found) - 1);
+        unit.y = __shfl_sync(0xffffffffu, unit_of[w].y, __ffs(found) - 1);
+      }
+      k -= __popc(heads[w]);
     }
-    const int a = s.first[u], n = s.last[u] - a + 1, shift = join_shift(n), dims = 128 >> shift;
-    const int4 head = s.piece[s.list[a]];
-    const int at = task - s.task[u], dim0 = (at & ((1 << shift) - 1)) * dims, groups0 = (min(head.w, QT) * G + 31) / 32;
-    const int half = (at >> shift) >= groups0, group = half ? 4 + (at >> shift) - groups0 : at >> shift;
-    const int r = (group & 3) * 32 + lane, nodes = half ? head.w - QT : min(head.w, QT), t = r / G;
-    __nv_bfloat16* const dst = p.out + (static_cast<long long>(head.y + half * QT + t) * p.H + head.z * G + (r - t * G)) * 128 + dim0;
-    const int stride = dims * 32 + 64;             // floats of a piece in the buffer: its dims, then maxima and sums
-    float M = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int base = 0; base < n; base += kTrJoinPieces) {
-      const int m = min(n - base, kTrJoinPieces);
-      __syncthreads();                             // the buffer has been read
-      if (tid == 0) mbar_expect_tx(&s.bar, m * stride * 4);
-      __syncwarp();
-      if (tid < m) {
-        const float* const from = p.partials + s.list[a + base + tid] * static_cast<long long>(kTrPartial) + group * kTrGroup;
-        tree_bulk_load(s.buf + tid * stride, from + dim0 * 32, dims * 128, &s.bar);
-        tree_bulk_load(s.buf + tid * stride + dims * 32, from + 128 * 32, 256, &s.bar);
-      }
-      if (!mbar_wait(&s.bar, loads & 1, &s.abort)) {
-        if (tid == 0) atomicExch(&g_status_tree, 1);
-        return;
-      }
-      ++loads;
-      // every warp for itself: the new maximum and sum; the weights are shared out
-      float top = M;
-#pragma unroll 4
-      for (int x = 0; x < m; ++x) top = fmaxf(top, s.buf[x * stride + dims * 32 + lane]);
-      const float ref = top == -INFINITY ? 0.f : top, was = fast_exp2(M - ref);
-      M = top;
-      sum *= was;
-#pragma unroll 4
-      for (int x = 0; x < m; ++x) {
-        const float w = fast_exp2(s.buf[x * stride + dims * 32 + lane] - ref);
-        sum = fmaf(s.buf[x * stride + dims * 32 + 32 + lane], w, sum);
-        if ((x & 3) == warp) s.weight[x][lane] = w;
-      }
-      __syncthreads();
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      // 4 dims of a warp at a time (with 16 dims in all, once: more pieces may follow)
-#pragma unroll 1
-      for (int d = warp * 4; d < dims; d += 16) {
+    const int at = task & ((8 << shift) - 1), group = at >> shift, half = group >> 2;
+    const int nodes = half ? nodes_all - QT : min(nodes_all, QT);
+    if ((group & 3) * 32 >= nodes * G) continue;
+    __syncthreads();                          // (the list and the buffer of the task in front have been read)
+    // its pieces: that CTA's second place, then first places up to the unit's last
+    int n = 1;
+    bool open = true;
+    if (tid == 0) s_list[0] = static_cast<short>(2 * c0 + 1);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = base ? o[i] * was : 0.f;
-#pragma unroll 2
-        for (int x = 0; x < m; ++x) {
-          const float w = s.weight[x][lane];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = fmaf(s.buf[x * stride + (d + i) * 32 + lane], w, o[i]);
+    for (int w = 0; w < kTrJoinWords; ++w) {
+      const int c = w * 32 + lane;
+      const unsigned after = __ballot_sync(0xffffffffu, c > c0), last = __ballot_sync(0xffffffffu, cont[w] == 2) & after;
+      unsigned mine = __ballot_sync(0xffffffffu, cont[w] != 0) & after;
+      if (last) mine &= last ^ (last - 1);    // up to the first of them
+      if (!open) mine = 0;
+      if (warp == 0 && (mine >> lane) & 1) s_list[n + __popc(mine & ((1u << lane) - 1))] = static_cast<short>(2 * c);
+      n += __popc(mine);
+      open = open && !last;
+    }
+    __syncthreads();
+    const int r = (group & 3) * 32 + lane, t = r / G;
+    const int dims_all = 128 >> shift, first_dim = (at & ((1 << shift) - 1)) * dims_all;
+    __nv_bfloat16* const dst = p.out + (static_cast<long long>(unit.x + half * QT + t) * p.H + unit.y * G + (r - t * G)) * 128;
+    // as many dims at a time as let all pieces into the buffer, at least 16
+    const int dims = min(dims_all, n <= 2 ? 128 : n <= 4 ? 64 : n <= 8 ? 32 : 16), stride = dims * 32 + 64;
+#pragma unroll 1
+    for (int dim0 = first_dim; dim0 < first_dim + dims_all; dim0 += dims) {
+      float M = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int base = 0; base < n; base += kTrJoinPieces) {
+        const int m = min(n - base, kTrJoinPieces);
+        if (loads) __syncthreads();           // the buffer has been read
+        if (tid == 0) mbar_expect_tx(&s_bar, m * stride * 4);
+        __syncwarp();
+        if (tid < m) {
+          // of a piece: its dims, then maxima and sums
+          const float* const from = p.partials + s_list[base + tid] * static_cast<long long>(kTrPartial) + group * kTrGroup;
+          tree_bulk_load(s_buf + tid * stride, from + dim0 * 32, dims * 128, &s_bar);
+          tree_bulk_load(s_buf + tid * stride + dims * 32, from + 128 * 32, 256, &s_bar);
         }
-        if (base + m == n && r < nodes * G)
-          *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+        if (!mbar_wait(&s_bar, loads & 1, &s_abort)) {
+          if (tid == 0) atomicExch(&g_status_tree, 1);
+          return;
+        }
+        ++loads;
+        // every warp for itself: the new maximum and sum; the weights are shared out
+        float top = M;
+#pragma unroll 1
+        for (int x = 0; x < m; ++x) top = fmaxf(top, s_buf[x * stride + dims * 32 + lane]);
+        const float ref = top == -INFINITY ? 0.f : top, was = fast_exp2(M - ref);
+        M = top;
+        sum *= was;
+#pragma unroll 1
+        for (int x = 0; x < m; ++x) {
+          const float w = fast_exp2(s_buf[x * stride + dims * 32 + lane] - ref);
+          sum = fmaf(s_buf[x * stride + dims * 32 + 32 + lane], w, sum);
+          if ((x & 3) == warp) s_weight[x][lane] = w;
+        }
+        __syncthreads();
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        // 4 dims of a warp at a time (more pieces follow with 16 dims only, which is once)
+#pragma unroll 1
+        for (int d = warp * 4; d < dims; d += 16) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = base ? o[i] * was : 0.f;
+#pragma unroll 2
+          for (int x = 0; x < m; ++x) {
+            const float w = s_weight[x][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(s_buf[x * stride + (d + i) * 32 + lane], w, o[i]);
+          }
+          if (base + m == n && r < nodes * G)
+            *reinterpret_cast<uint2*>(dst + dim0 + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
+        }
       }
     }
   }
 }
 
 // Workspace: the pieces' records, then two places of partial results per CTA.
-static int64_t tree_pieces_bytes(int ctas) { return (static_cast<int64_t>(ctas) * 2 * sizeof(TreePiece) + 255) / 256 * 256; }
-static int64_t tree_workspace(int ctas) { return tree_pieces_bytes(ctas) + static_cast<int64_t>(ctas) * 2 * kTrPartial * 4; }
+constexpr int64_t kTrPiecesBytes = (sizeof(TreePieces) + 255) / 256 * 256;
+static int64_t tree_workspace(int ctas) { return kTrPiecesBytes + static_cast<int64_t>(ctas) * 2 * kTrPartial * 4; }
 
 int read_status_tree() {
   int v = 0;
@@ -948,8 +951,8 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   if (line >= 2147483648.0) return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
   const int grid = sm_count();
   if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
-  p.pieces = static_cast<int*>(workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + tree_pieces_bytes(grid));
+  p.pieces = static_cast<TreePieces*>(workspace);
+  p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTrPiecesBytes);
   CUtensorMap map_q, map_k, map_v, map_k16, map_v16;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * block_size, row = static_cast<uint64_t>(num_kv_heads) * 128;
   int rc = make_tokens_heads_map(&map_q, q, static_cast<uint64_t>(total_q), num_heads, static_cast<uint64_t>(q_row_stride), 128 / G, G);

@@ -20,7 +20,7 @@ struct TreeParams {
   int mask_words;                    // 32-bit words of a row
   int batch, total_q, H, Hkv, G;
   float scale_log2;
-  int* pieces;                       // [2 * CTAs] records of cut units (TreePiece)
+  struct TreePieces* pieces;         // records of cut units
   float* partials;                   // [2 * CTAs] partial results
 };
 
