@@ -16,6 +16,8 @@
 // The halves are two softmax chains.  Work is a row of steps that they take in strict turn, across the units' borders: a step is a
 // key tile of a unit with at most 128 rows (the output warpgroup joins what the halves have of it), or a key tile for one of the
 // two Q tiles of a larger unit.
+// kCluster, for few units: a thread-block cluster of 8 CTAs has a unit and shares its key tiles out; their partial results are joined
+// through distributed shared memory, each CTA joining and writing 16 of the dims, so there is no second launch.
 // TMEM: S [0,128)  P_A [128,192)  P_B [192,256)  O_A [256,384)  O_B [384,512).  Both halves' scores go through one S: a row is in
 // its thread's registers 200 cycles after the product, and then the next step's product may run.  With an S of its own in
 // which P replaced the scores, a half's next S had to wait for its P V: a chain of 3740 cycles a tile at 256 rows, of which the
@@ -148,6 +150,25 @@ struct TreeRows {
   }
 };
 
+__device__ __forceinline__ void tree_cluster_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Shared-memory address of CTA `rank` of the cluster that corresponds to this CTA's `addr`.
+__device__ __forceinline__ uint32_t tree_cluster_addr(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void tree_cluster_store(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+// What the CTAs of a cluster send one another, in the room of the rings: for each of them 16 dims and then maxima and sums of 256 rows.
+constexpr int kTrCluster = 8;
+constexpr int kTrInbox = (16 + 2) * 256;      // floats of one sender
+
+template <bool kCluster>
 __global__ void __launch_bounds__(kTrThreads, 1)
 tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_k16,
@@ -194,6 +215,29 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     s_at[0][1] = s_at[0][2] = s_at[1][1] = s_at[1][2] = 0;
   }
   __syncthreads();
+  int c_nodes = 0, c_row = 0, c_head = 0, c_tiles = 0;       // kCluster: the cluster's unit
+  const int c_rank = blockIdx.x % kTrCluster;
+  if constexpr (kCluster) {
+    // sequence i owns blocks of nodes [cu_q[i] / (2 * QT) + i, ...); there are few sequences
+    const int x = static_cast<int>(blockIdx.x / kTrCluster), slot = x / p.Hkv;
+    c_head = x - slot * p.Hkv;
+    int seq = 0;
+#pragma unroll 1
+    for (int i = 1; i < p.batch; ++i)
+      if (max(0, min(__ldg(p.cu_q + i), p.total_q)) / (2 * QT) + i <= slot) seq = i;
+    const TreeSeq s = tree_seq(p, QT, seq);
+    const int block = slot - (s.q_begin / (2 * QT) + seq), node0 = block * 2 * QT;
+    c_nodes = block >= 0 ? min(s.nodes - node0, 2 * QT) : 0;
+    c_row = s.q_begin + node0;
+    c_tiles = s.tiles;
+    if (c_nodes > 0 && tid == 0) {
+      s_bare = c_rank == 0 && c_tiles == 0;
+      s_at[0][0] = s_at[1][0] = c_tiles > 0 ? seq : p.batch;
+      s_at[0][1] = s_at[1][1] = block * p.Hkv + c_head;
+      s_at[0][2] = c_tiles * c_rank / kTrCluster;
+      s_at[1][2] = c_tiles * (c_rank + 1) / kTrCluster;
+    }
+  } else
   // The CTA's share of the line.  (Lengths ahead of the wait below: no kernel that lets this one start early writes them.)
   // With up to a block of sequences one sum over them gives the total and every sequence's place; larger batches take two.
   {
@@ -253,9 +297,13 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   __syncthreads();
   volatile int* abort_flag = &s_abort;
   uint32_t tmem = 0;
+  bool met = false;               // kCluster: this thread has been through the first meeting
   if (warp > 0) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (s_bare) {
+    if (kCluster && s_bare) {
+      for (int e = tid - 32; e < c_nodes * G * 16; e += kTrThreads - 32)
+        reinterpret_cast<uint4*>(p.out + (static_cast<long long>(c_row + e / (G * 16)) * p.H + c_head * G) * 128)[e % (G * 16)] = make_uint4(0, 0, 0, 0);
+    } else if (s_bare) {
       // sequences with nodes and no keys: zeros
 #pragma unroll 1
       for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
@@ -357,15 +405,18 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         }
       }
       if (!started) asm volatile("griddepcontrol.wait;" ::: "memory");
-      p.pieces->cont[blockIdx.x] = cont;
-      p.pieces->head[blockIdx.x] = head;
-      p.pieces->unit[blockIdx.x] = head_unit;
+      if constexpr (!kCluster) {
+        p.pieces->cont[blockIdx.x] = cont;
+        p.pieces->head[blockIdx.x] = head;
+        p.pieces->unit[blockIdx.x] = head_unit;
+      }
       if (ok) {
         const int is = n_pub % kTrItems;
         if (t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) {
           s_item[is].seq = -1;
           mbar_arrive(&bar_item_full[is]);
-          t2_wait_timed(&bar_item_empty[is], (n_pub / kTrItems) & 1, abort_flag);      // every role has taken it
+          // every role has taken it (kCluster: the output warps do so behind the meeting that this warp is to come to)
+          if (!kCluster) t2_wait_timed(&bar_item_empty[is], (n_pub / kTrItems) & 1, abort_flag);
         }
       }
     } else if (warp == 1 && lane == 0) {
@@ -668,6 +719,16 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         if (!ok) break;
         tc::fence_after_sync();
         const int tile_nodes = turn == 0 ? min(it.nodes, QT) : it.nodes - QT;
+        if constexpr (kCluster) {
+          // (the last turn waited for is the CTA's last product: nothing reads the rings any more)
+          if (turn == 0) {
+            if (!it.split) {
+              if (!t2_wait(&bar_o_final[it.turn ^ 1], nf[it.turn ^ 1] & 1, abort_flag)) { ok = false; break; }
+            }
+            tree_cluster_sync();
+            met = true;
+          }
+        }
         if (quarter * 32 < tile_nodes * G) {
           const float M = fmaxf(m[0], m[1]);
           float wa = M == -INFINITY ? 0.f : fast_exp2(m[0] - M), wb = M == -INFINITY ? 0.f : fast_exp2(m[1] - M);
@@ -675,8 +736,15 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
           const bool row_ok = r < tile_nodes * G;
           const int t = r / G;
           __nv_bfloat16* const dst = p.out + (static_cast<long long>(it.q_row + turn * QT + t) * p.H + it.h * G + (r - t * G)) * 128;
-          float* const part = it.partial < 0 ? nullptr : p.partials + static_cast<long long>(it.partial) * kTrPartial + (turn * 4 + quarter) * kTrGroup + lane;
-          if (part) {
+          float* const part = kCluster || it.partial < 0 ? nullptr : p.partials + static_cast<long long>(it.partial) * kTrPartial + (turn * 4 + quarter) * kTrGroup + lane;
+          const uint32_t inbox = smem_u32(smem) + (c_rank * kTrInbox + turn * 128 + r) * 4;
+          if constexpr (kCluster) {
+#pragma unroll 1
+            for (int x = 0; x < kTrCluster; ++x) {
+              tree_cluster_store(tree_cluster_addr(inbox + 16 * 1024, x), M);
+              tree_cluster_store(tree_cluster_addr(inbox + 17 * 1024, x), sum);
+            }
+          } else if (part) {
             part[128 * 32] = M;
             part[129 * 32] = sum;
           } else {
@@ -699,7 +767,11 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
             tc::wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), wb, __uint_as_float(a[i]) * wa));
-            if (part) {
+            if constexpr (kCluster) {
+              const uint32_t to = tree_cluster_addr(inbox, cch);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) tree_cluster_store(to + i * 1024, __uint_as_float(a[i]));
+            } else if (part) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) part[(cch * 16 + i) * 32] = __uint_as_float(a[i]);
             } else if (row_ok) {
@@ -725,6 +797,36 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     }
   }
 
+  if constexpr (kCluster) {
+    if (!met) tree_cluster_sync();             // (output warps that had an item have been here before)
+    tree_cluster_sync();
+    // all partial results are here: a thread joins 8 of this CTA's 16 dims of a row
+    const float* const inbox = reinterpret_cast<const float*>(smem);
+    const int row = tid & 255, half = row >> 7, r = row & 127, t = r / G, node = half * QT + t;
+    if (r < QT * G && node < c_nodes && c_tiles > 0) {
+      float M = -INFINITY;
+#pragma unroll 1
+      for (int x = 0; x < kTrCluster; ++x)
+        if (c_tiles * (x + 1) / kTrCluster > c_tiles * x / kTrCluster) M = fmaxf(M, inbox[x * kTrInbox + 16 * 256 + row]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int x = 0; x < kTrCluster; ++x) {
+        if (c_tiles * (x + 1) / kTrCluster == c_tiles * x / kTrCluster) continue;
+        const float w = fast_exp2(inbox[x * kTrInbox + 16 * 256 + row] - ref);
+        sum = fmaf(inbox[x * kTrInbox + 17 * 256 + row], w, sum);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = fmaf(inbox[x * kTrInbox + ((tid >> 8) * 8 + i) * 256 + row], w, o[i]);
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      uint4 v;
+      v.x = pack_bf16(o[0] * inv, o[1] * inv);
+      v.y = pack_bf16(o[2] * inv, o[3] * inv);
+      v.z = pack_bf16(o[4] * inv, o[5] * inv);
+      v.w = pack_bf16(o[6] * inv, o[7] * inv);
+      reinterpret_cast<uint4*>(p.out + (static_cast<long long>(c_row + node) * p.H + c_head * G + (r - t * G)) * 128)[c_rank * 2 + (tid >> 8)] = v;
+    }
+  }
   // ---- teardown: everyone meets, then the allocating warp frees TMEM ----
   tc::fence_before_sync();
   __syncthreads();
@@ -873,6 +975,47 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
   }
 }
 
+constexpr size_t kTrSmem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTile;
+// Table width (in key tiles) up to which few units go to clusters.
+constexpr int kTrClusterTiles = 64;
+
+template <bool kCluster>
+static int tree_configure() {
+  static std::atomic<size_t> configured[kMaxDevices];
+  return ensure_dynamic_smem(reinterpret_cast<const void*>(tree_attn_kernel<kCluster>), kTrSmem, configured, "tree_attn: cudaFuncSetAttribute");
+}
+static void tree_cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, unsigned clusters, cudaStream_t stream) {
+  cfg->gridDim = dim3(clusters * kTrCluster);
+  cfg->blockDim = dim3(kTrThreads);
+  cfg->dynamicSmemBytes = kTrSmem;
+  cfg->stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kTrCluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 2;
+}
+// How many clusters the current device holds at a time (0: not known).
+static int tree_clusters_on_chip() {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
+  if ((n = known[dev].load(std::memory_order_acquire)) > 0) return n;
+  if (tree_configure<true>()) return 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  tree_cluster_config(&cfg, attr, 1, nullptr);
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, tree_attn_kernel<true>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  known[dev].store(n, std::memory_order_release);
+  return n;
+}
+
 // Workspace: the pieces' records, then two places of partial results per CTA.
 constexpr int64_t kTrPiecesBytes = (sizeof(TreePieces) + 255) / 256 * 256;
 static int64_t tree_workspace(int ctas) { return kTrPiecesBytes + static_cast<int64_t>(ctas) * 2 * kTrPartial * 4; }
@@ -961,11 +1104,21 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   if (!rc) rc = make_tokens_heads_map(&map_k16, k_cache, rows, num_kv_heads, row, 16);
   if (!rc) rc = make_tokens_heads_map(&map_v16, v_cache, rows, num_kv_heads, row, 16);
   if (rc) return rc;
-  const size_t smem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTile;
-  static std::atomic<size_t> configured[kMaxDevices];
-  rc = ensure_dynamic_smem(reinterpret_cast<const void*>(tree_attn_kernel), smem, configured, "tree_attn: cudaFuncSetAttribute");
+  // few units: a cluster each, one launch
+  const long long units = (static_cast<long long>(total_q) / (2 * (128 / G)) + batch) * num_kv_heads;
+  if (static_cast<long long>(bt_cols) * (block_size / kTrKv) <= kTrClusterTiles && units <= tree_clusters_on_chip()) {
+    rc = tree_configure<true>();
+    if (rc) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    tree_cluster_config(&cfg, attr, static_cast<unsigned>(units), static_cast<cudaStream_t>(stream));
+    const cudaError_t le = cudaLaunchKernelEx(&cfg, tree_attn_kernel<true>, p, map_q, map_k, map_v, map_k16, map_v16);
+    g_launches.fetch_add(1);
+    return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn(cluster) launch");
+  }
+  rc = tree_configure<false>();
   if (rc) return rc;
-  cudaError_t le = launch_early(tree_attn_kernel, grid, kTrThreads, smem, static_cast<cudaStream_t>(stream), p, map_q, map_k, map_v, map_k16, map_v16);
+  cudaError_t le = launch_early(tree_attn_kernel<false>, grid, kTrThreads, kTrSmem, static_cast<cudaStream_t>(stream), p, map_q, map_k, map_v, map_k16, map_v16);
   g_launches.fetch_add(1);
   rc = check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn launch");
   if (rc || grid < 2) return rc;
