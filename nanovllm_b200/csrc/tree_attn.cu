@@ -40,8 +40,10 @@ constexpr int kTrThreads = 512;
 constexpr int kTrRingK = 2, kTrRingV = 3;     // tiles of K and V in shared memory
 constexpr int kTrItems = 4;                   // items in flight
 constexpr float kTrRescale = 8.0f;
-// The line's measure: cost of a key tile with the halves sharing it out, with a Q tile each, and of a unit by itself.
-constexpr int kTrCostSplit = 4, kTrCostPair = 5, kTrCostUnit = 10;
+// The line's measure: cost of a key tile and of a unit by itself, with at most QT nodes (a step per tile) and with more (two).  Fitted to
+// the cycles of a CTA's P V thread: 256 chains of 4 nodes, bound by memory, 2210 a tile and 2380 a unit; 13 ragged trees about
+// 1300 and 3300 a tile of either kind; 128 trees of 64 nodes 3090 a tile and 11300 a unit.
+constexpr int kTrTileSplit = 4, kTrUnitSplit = 5, kTrTilePair = 7, kTrUnitPair = 24;
 // Partial results of one piece: 8 groups of 32 rows, each [128 dims][32 rows] and [max, sum][32 rows] in fp32, so that both kernels
 // move whole lines with a row per lane.
 constexpr int kTrGroup = 130 * 32;
@@ -94,19 +96,20 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int QT, int i) 
 // (32 bits: the host refuses geometries whose line might be longer)
 __device__ __forceinline__ unsigned tree_cost(const TreeSeq& s, int Hkv) {
   if (s.blocks == 0) return 0;
-  return Hkv * (s.blocks * (s.tiles * kTrCostPair + kTrCostUnit) - (s.last_split ? s.tiles * (kTrCostPair - kTrCostSplit) : 0));
+  return Hkv * ((s.blocks - s.last_split) * (s.tiles * kTrTilePair + kTrUnitPair) + s.last_split * (s.tiles * kTrTileSplit + kTrUnitSplit));
 }
 // Place `off` of a sequence's part of the line: unit (block * Hkv + head) and key tile.
 __device__ __forceinline__ void tree_locate(const TreeSeq& s, int Hkv, unsigned off, int& unit, int& tile) {
-  const unsigned pair = s.tiles * kTrCostPair + kTrCostUnit;
+  const unsigned pair = s.tiles * kTrTilePair + kTrUnitPair;
   const unsigned block = s.blocks == 1 ? 0 : min(off / (pair * Hkv), static_cast<unsigned>(s.blocks - 1));
   off -= block * pair * Hkv;
-  const unsigned w = block == s.blocks - 1 && s.last_split ? kTrCostSplit : kTrCostPair;
-  const unsigned one = s.tiles * w + kTrCostUnit;
+  const bool split = block == s.blocks - 1 && s.last_split;
+  const unsigned w = split ? kTrTileSplit : kTrTilePair, start = split ? kTrUnitSplit : kTrUnitPair;
+  const unsigned one = s.tiles * w + start;
   const unsigned h = off / one;
   off -= h * one;
   unit = static_cast<int>(block * Hkv + h);
-  tile = static_cast<int>(off < kTrCostUnit ? 0 : (off - kTrCostUnit) / w);
+  tile = static_cast<int>(off < start ? 0 : (off - start) / w);
 }
 
 // A key tile of K or V into its place: in one box per half of the dims; of a sequence's last tile only what it has (`left` keys), in
@@ -1090,7 +1093,7 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.scale_log2 = scale * 1.4426950408889634f;
   // the longest that the line of key tiles can be (table widths are all that the host knows of the lengths)
   const double line = static_cast<double>(num_kv_heads) * (total_q / (2 * (128 / G)) + batch) *
-                      (static_cast<double>(bt_cols) * (block_size / kTrKv) * kTrCostPair + kTrCostUnit);
+                      (static_cast<double>(bt_cols) * (block_size / kTrKv) * kTrTilePair + kTrUnitPair);
   if (line >= 2147483648.0) return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
   const int grid = sm_count();
   if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
