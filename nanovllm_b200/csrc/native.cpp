@@ -590,6 +590,29 @@ bool optional_tensor(PyObject* o, const char* what, const Tensor** t) {
 }
 constexpr int64_t kMost = 0x7fffffff;
 
+// Several outputs of one call out of one allocation: five to seven of their own cost the host as much as the launch.  Each
+// begins at a multiple of 16 bytes.
+struct Outputs {
+  struct One { at::DimVector sizes; at::ScalarType type; int64_t at; };
+  c10::SmallVector<One, 7> all;
+  int64_t bytes = 0;
+  Tensor base;
+  void want(at::IntArrayRef sizes, at::ScalarType type) {
+    all.push_back({at::DimVector(sizes), type, bytes});
+    int64_t n = static_cast<int64_t>(c10::elementSize(type));
+    for (const int64_t s : sizes) n *= s;
+    bytes += (n + 15) / 16 * 16;
+  }
+  void allocate(at::Device device) { base = at::detail::empty_cuda({bytes}, at::kByte, device, std::nullopt); }
+  Tensor get(int i) const {
+    const One& o = all[i];
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(o.type));
+    impl->set_storage_offset(o.at / static_cast<int64_t>(c10::elementSize(o.type)));
+    impl->set_sizes_contiguous(o.sizes);
+    return Tensor(std::move(impl));
+  }
+};
+
 // The allocator's state: tables (requests, columns), owned (requests), free_blocks (blocks), pool (2).
 bool check_block_state(const Tensor& tables, const Tensor& owned, const Tensor& free_blocks, const Tensor& pool) {
   const char* bad = nullptr;
@@ -634,15 +657,16 @@ PyObject* py_step_tables(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
   Tensor o[7];
   int64_t buffer_rows = b;
   if (a[11] == Py_None) {
-    const auto dev = t[0]->device();
-    const auto make = [&](at::IntArrayRef sizes, at::ScalarType type) { return at::detail::empty_cuda(sizes, type, dev, std::nullopt); };
-    o[0] = make({b + 1}, at::kInt);
-    o[1] = make({b + 1}, at::kInt);
-    o[2] = make({b}, at::kInt);
-    o[3] = make({num_tokens}, at::kInt);
-    o[4] = make({num_tokens}, at::kLong);
-    o[5] = make({b, cols}, at::kInt);
-    if (parents) o[6] = make({num_tokens, words}, at::kLong);
+    Outputs outs;
+    outs.want({b + 1}, at::kInt);
+    outs.want({b + 1}, at::kInt);
+    outs.want({b}, at::kInt);
+    outs.want({num_tokens}, at::kInt);
+    outs.want({num_tokens}, at::kLong);
+    outs.want({b, cols}, at::kInt);
+    if (parents) outs.want({num_tokens, words}, at::kLong);
+    outs.allocate(t[0]->device());
+    for (int i = 0; i < (parents ? 7 : 6); ++i) o[i] = outs.get(i);
   } else {
     Ref outs(PySequence_Fast(a[11], "out must be a sequence of tensors"));
     if (!outs.o) return nullptr;
@@ -776,9 +800,13 @@ PyObject* py_accept_tree(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
           "cu_seqlens_q, cached_lens and context_lens must be int32, one per sequence (cu_seqlens_q one more)");
   REQUIRE(max_path >= 1 && n <= kMost && b <= kMost, "max_path must be at least 1");
   const c10::cuda::CUDAGuard guard(t[0]->device());
-  const auto dev = t[0]->device();
-  Tensor o[4] = {at::detail::empty_cuda({b}, at::kInt, dev, std::nullopt), at::detail::empty_cuda({b, max_path}, at::kInt, dev, std::nullopt),
-                 at::detail::empty_cuda({b, max_path}, at::kLong, dev, std::nullopt), at::detail::empty_cuda({b}, at::kInt, dev, std::nullopt)};
+  Outputs outs;
+  outs.want({b}, at::kInt);
+  outs.want({b, max_path}, at::kInt);
+  outs.want({b, max_path}, at::kLong);
+  outs.want({b}, at::kInt);
+  outs.allocate(t[0]->device());
+  Tensor o[4] = {outs.get(0), outs.get(1), outs.get(2), outs.get(3)};
   LAUNCH(b200_accept_tree(longs(t[0]), longs(t[1]), ints(t[2]), ints(t[3]), ints(t[4]), ints(t[5]), static_cast<int32_t>(b),
                           static_cast<int32_t>(n), max_path, ints(&o[0]), ints(&o[1]), longs(&o[2]), ints(&o[3]), stream_ptr()));
   PyObject* res = PyTuple_New(4);
