@@ -18,7 +18,7 @@
 namespace b200 {
 extern std::atomic<long long> g_launches;
 
-constexpr int kStepThreads = 1024;
+constexpr int kStepThreads = 512;
 constexpr int kStepCtas = 8;
 constexpr int kStepMaxBatch = 4096;      // what the scan keeps in shared memory
 constexpr int kStepMaxWords = 4;         // trees of up to 256 nodes
@@ -38,32 +38,36 @@ struct StepParams {
   int hash_slots;                                  // power of two, 0 without rows
 };
 
-// Sums over the block: each thread's own prefix (exclusive) and the total.  All threads take part.
-template <typename T>
-__device__ __forceinline__ T block_scan(T v, T* scratch /* [33] */, T& total) {
+// Sums over the block of two numbers: each thread's own prefixes (exclusive) and the totals.  All threads take part.
+struct StepSum {
+  long long a;
+  int b;
+};
+__device__ __forceinline__ StepSum block_scan(StepSum v, StepSum* scratch /* [kStepThreads / 32] */, StepSum& total) {
+  constexpr int kWarps = kStepThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  T x = v;
+  StepSum x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const T y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    const long long a = __shfl_up_sync(0xffffffffu, x.a, o);
+    const int b = __shfl_up_sync(0xffffffffu, x.b, o);
+    if (lane >= o) { x.a += a; x.b += b; }
   }
   if (lane == 31) scratch[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    T w = scratch[lane];
+  StepSum w = lane < kWarps ? scratch[lane] : StepSum{0, 0};      // (every warp for itself: one barrier less)
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const T y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    scratch[lane] = w;
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, w.a, o);
+    const int b = __shfl_up_sync(0xffffffffu, w.b, o);
+    if (lane >= o) { w.a += a; w.b += b; }
   }
-  __syncthreads();
-  const T before = warp ? scratch[warp - 1] : T(0);
-  total = scratch[31];
-  __syncthreads();
-  return before + x - v;
+  const int front = max(warp - 1, 0);
+  const long long fa = __shfl_sync(0xffffffffu, w.a, front);
+  const int fb = __shfl_sync(0xffffffffu, w.b, front);
+  total.a = __shfl_sync(0xffffffffu, w.a, kWarps - 1);
+  total.b = __shfl_sync(0xffffffffu, w.b, kWarps - 1);
+  return {(warp ? fa : 0) + x.a - v.a, (warp ? fb : 0) + x.b - v.b};
 }
 
 // Marks, for each row that occurs in rows[0 .. batch), its first place: open addressing with as many slots as twice the batch.
@@ -104,34 +108,44 @@ __global__ void __cluster_dims__(kStepCtas, 1, 1) __launch_bounds__(kStepThreads
   int* const s_row = s_top + p.batch;           // [batch]
   int* const s_keys = s_row + p.batch;          // [hash_slots]
   int* const s_firsts = s_keys + p.hash_slots;  // [hash_slots]
-  __shared__ long long scratch_l[33];
-  __shared__ int scratch_i[33];
+  __shared__ StepSum scratch[2][kStepThreads / 32];
+  __shared__ int s_granted;
   const int tid = threadIdx.x, rank = blockIdx.x;
-  if (p.rows) hash_rows(p.rows, p.batch, p.hash_slots, s_keys, s_firsts);
+  // What stands in the way is one load behind the other, so the first ones go out together: the thread's sequence, and the
+  // parents of its tokens on their way into L1.
   const int n_free = max(0, min(p.pool[0], p.num_blocks));
-  long long tokens = 0;
-  int wanted = 0, granted = 0, left_out = 0;
-  long long keys_so_far = 0;
+  const bool live0 = tid < p.batch;
+  const int row0 = live0 ? (p.rows ? p.rows[tid] : tid) : -1, cached0 = live0 ? p.cached[tid] : 0, fresh0 = live0 ? p.fresh[tid] : 0;
+  if (p.masks)
+    for (int t = rank * kStepThreads + tid; t < p.num_tokens; t += kStepCtas * kStepThreads)
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.parents + t));
+  const int owned0 = row0 >= 0 && row0 < p.max_requests ? p.owned[row0] : 0;
+  if (tid == 0) s_granted = 0;
+  if (p.rows) hash_rows(p.rows, p.batch, p.hash_slots, s_keys, s_firsts);
+  else __syncthreads();
+  long long tokens = 0, keys_so_far = 0;
+  int wanted = 0, left_out = 0;
+#pragma unroll 1
   for (int base = 0; base < p.batch; base += kStepThreads) {
     const int i = base + tid;
     const bool live = i < p.batch;
-    const int row = live ? (p.rows ? p.rows[i] : i) : -1;
-    const int cached = live ? max(p.cached[i], 0) : 0, fresh = live ? max(p.fresh[i], 0) : 0;
+    const int row = base == 0 ? row0 : live ? (p.rows ? p.rows[i] : i) : -1;
+    const int cached = max(base == 0 ? cached0 : live ? p.cached[i] : 0, 0), fresh = max(base == 0 ? fresh0 : live ? p.fresh[i] : 0, 0);
     const long long len = static_cast<long long>(cached) + fresh;
     bool ok = live && row >= 0 && row < p.max_requests && len <= INT_MAX - p.block_size;
     if (ok && p.rows) ok = first_place(row, i, p.hash_slots, s_keys, s_firsts);
-    const int held = ok ? max(0, min(p.owned[row], p.table_cols)) : 0;
+    const int held = ok ? max(0, min(base == 0 ? owned0 : p.owned[row], p.table_cols)) : 0;
     const int need = ok ? (static_cast<int>(len) + p.block_size - 1) / p.block_size : 0;
     ok = ok && need <= p.table_cols && !(p.masks && fresh > 64 * p.mask_words);
-    long long total_l;
-    const long long t0 = tokens + block_scan<long long>(fresh, scratch_l, total_l);
-    tokens += total_l;
-    ok = ok && t0 + fresh <= p.num_tokens;
-    const int want = ok ? max(need - held, 0) : 0;
-    int total_i;
-    const int before = wanted + block_scan<int>(want, scratch_i, total_i);
-    wanted += total_i;
-    ok = ok && (want == 0 || before + want <= n_free);
+    // (whether a sequence's tokens fit is known with the first sum only; what it would have wanted must not count then, so
+    // those behind the last token that fits are cut off: the sums grow)
+    StepSum total;
+    const StepSum at = block_scan({fresh, ok ? max(need - held, 0) : 0}, scratch[0], total);
+    const long long t0 = tokens + at.a;
+    const int want = ok ? max(need - held, 0) : 0, before = wanted + at.b;
+    tokens += total.a;
+    wanted += total.b;
+    ok = ok && t0 + fresh <= p.num_tokens && (want == 0 || before + want <= n_free);
     if (live) {
       s_cu[i] = static_cast<int>(min(t0, static_cast<long long>(p.num_tokens)));
       s_cached[i] = cached;
@@ -141,19 +155,19 @@ __global__ void __cluster_dims__(kStepCtas, 1, 1) __launch_bounds__(kStepThreads
       s_row[i] = row;
     }
     if (rank == 0) {
+      // (what is granted is what comes first of what is wanted)
       const int context = ok ? static_cast<int>(len) : 0;
-      const long long k0 = keys_so_far + block_scan<long long>(context, scratch_l, total_l);
-      keys_so_far += total_l;
-      block_scan<int>(ok ? want : 0, scratch_i, total_i);
-      granted += total_i;
-      block_scan<int>(live && !ok, scratch_i, total_i);
-      left_out += total_i;
+      const StepSum k = block_scan({context, live && !ok ? 1 : 0}, scratch[1], total);
       if (live) {
         p.cu_q[i] = s_cu[i];
-        p.cu_k[i] = static_cast<int>(k0);
+        p.cu_k[i] = static_cast<int>(keys_so_far + k.a);
         p.context[i] = context;
       }
+      keys_so_far += total.a;
+      left_out += total.b;
+      if (ok && want > 0) atomicMax(&s_granted, before + want);
     }
+    __syncthreads();
   }
   const int all = static_cast<int>(min(tokens, static_cast<long long>(p.num_tokens)));
   if (tid == 0) s_cu[p.batch] = all;
@@ -227,7 +241,7 @@ __global__ void __cluster_dims__(kStepCtas, 1, 1) __launch_bounds__(kStepThreads
     for (int i = tid; i < p.batch; i += kStepThreads)
       if (s_need[i] > s_held[i]) p.owned[s_row[i]] = s_need[i];
     if (tid == 0) {
-      p.pool[0] = n_free - granted;
+      p.pool[0] = n_free - s_granted;
       p.pool[1] = left_out;
     }
   }
@@ -252,29 +266,34 @@ __global__ void __launch_bounds__(kStepThreads, 1) release_blocks_kernel(const R
   int* const s_row = s_keep + p.batch;          // [batch]
   int* const s_keys = s_row + p.batch;
   int* const s_firsts = s_keys + p.hash_slots;
-  __shared__ int scratch[33];
+  __shared__ StepSum scratch[kStepThreads / 32];
   const int tid = threadIdx.x;
-  if (p.rows) hash_rows(p.rows, p.batch, p.hash_slots, s_keys, s_firsts);
   const int n_free = max(0, min(p.pool[0], p.num_blocks));
+  const bool live0 = tid < p.batch;
+  const int row0 = live0 ? (p.rows ? p.rows[tid] : tid) : -1, len0 = live0 ? p.keep_lens[tid] : 0;
+  const int owned0 = row0 >= 0 && row0 < p.max_requests ? p.owned[row0] : 0;
+  if (p.rows) hash_rows(p.rows, p.batch, p.hash_slots, s_keys, s_firsts);
   int back = 0;
+#pragma unroll 1
   for (int base = 0; base < p.batch; base += kStepThreads) {
     const int i = base + tid;
     const bool live = i < p.batch;
-    const int row = live ? (p.rows ? p.rows[i] : i) : -1;
+    const int row = base == 0 ? row0 : live ? (p.rows ? p.rows[i] : i) : -1;
     bool ok = row >= 0 && row < p.max_requests;
     if (ok && p.rows) ok = first_place(row, i, p.hash_slots, s_keys, s_firsts);
-    const int held = ok ? max(0, min(p.owned[row], p.table_cols)) : 0;
-    const int len = live ? max(p.keep_lens[i], 0) : 0;
+    const int held = ok ? max(0, min(base == 0 ? owned0 : p.owned[row], p.table_cols)) : 0;
+    const int len = max(base == 0 ? len0 : live ? p.keep_lens[i] : 0, 0);
     const int keep = min(len / p.block_size + (len % p.block_size != 0), held);
-    int total;
-    const int before = back + block_scan<int>(held - keep, scratch, total);
-    back += total;
+    StepSum total;
+    const int before = back + block_scan({0, held - keep}, scratch, total).b;
+    back += total.b;
     if (live) {
       s_before[i] = before;
       s_keep[i] = keep;
       s_row[i] = row;
       if (keep < held) p.owned[row] = keep;      // (rows are distinct where they release anything)
     }
+    __syncthreads();
   }
   if (tid == 0) s_before[p.batch] = back;
   __syncthreads();
