@@ -121,7 +121,7 @@ int b200_device_status(void) {
     cudaError_t e = cudaGetLastError();
     return b200::check_cuda(e == cudaSuccess ? cudaErrorUnknown : e, "device_status: cudaDeviceSynchronize");
   }
-  const int sd = b200::read_status_decode() | b200::read_status_decode_cluster(), sm = b200::read_status_prefill_mma(), st = b200::read_status_prefill_tc2(), tr = b200::read_status_tree();
+  const int sd = b200::read_status_decode() | b200::read_status_decode_cluster(), sm = b200::read_status_prefill_mma(), st = b200::read_status_prefill_tc2(), tr = b200::read_status_tree() | b200::read_status_tree_small();
   if (sd || sm || st || tr) {
     // Report once and recover: clear the status words and the library's own launch-to-launch state, so that the
     // next call of this function speaks about later launches only and the next prefill starts from ticket 0.
@@ -130,6 +130,7 @@ int b200_device_status(void) {
     if (!rc) rc = b200::reset_state_prefill_mma();
     if (!rc) rc = b200::reset_state_prefill_tc2();
     if (!rc) rc = b200::reset_state_tree();
+    if (!rc) rc = b200::reset_state_tree_small();
     if (rc) return rc;
     return b200::set_error(b200::kErrTimeout,
                            "a bounded device-side wait gave up (decode=%d prefill mma.sync=%d prefill tcgen05=%d tree=%d); the "

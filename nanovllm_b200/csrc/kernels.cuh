@@ -54,6 +54,8 @@ int read_status_prefill_mma();
 int read_status_prefill_tc2();
 int read_status_tree();
 int reset_state_tree();
+int read_status_tree_small();
+int reset_state_tree_small();
 int reset_state_decode();
 int reset_state_decode_cluster();
 int reset_state_prefill_mma();

@@ -43,11 +43,10 @@ constexpr float kTrRescale = 8.0f;
 // The line's measure: cost of a key tile and of a unit by itself, with at most QT nodes (a step per tile) and with more (two).  Fitted to
 // the cycles of a CTA's P V thread: 256 chains of 4 nodes, bound by memory, 2210 a tile and 2380 a unit; 13 ragged trees about
 // 1300 and 3300 a tile of either kind; 128 trees of 64 nodes 3090 a tile and 11300 a unit.
-constexpr int kTrTileSplit = 4, kTrUnitSplit = 5, kTrTilePair = 7, kTrUnitPair = 24;
-// Partial results of one piece: 8 groups of 32 rows, each [128 dims][32 rows] and [max, sum][32 rows] in fp32, so that both kernels
-// move whole lines with a row per lane.
-constexpr int kTrGroup = 130 * 32;
-constexpr int kTrPartial = 8 * kTrGroup;      // floats
+struct TcLine {
+  static constexpr int kKeys = kTrKv;
+  static constexpr int kTileSplit = 4, kUnitSplit = 5, kTilePair = 7, kUnitPair = 24;
+};
 
 static __device__ int g_status_tree = 0;
 
@@ -69,49 +68,6 @@ __device__ __forceinline__ void tree_bulk_load(void* dst, const void* src, uint3
                ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-// What a cut unit's pieces are, for the join.  A CTA's share can begin within a unit (its partial results go to place 2 * CTA) and end
-// within one that it began (place 2 * CTA + 1).  Every CTA writes its entries.
-constexpr int kTrMaxCtas = 160;               // (a B200 has 148 multiprocessors)
-struct TreePieces {
-  int head[kTrMaxCtas];                       // nodes of the unit that the share ends within, 0: none
-  int cont[kTrMaxCtas];                       // the share begins within a unit: 1, or 2 if it has the unit's last tile, too; 0: it does not
-  int2 unit[kTrMaxCtas];                      // where head is set: the unit's first row, its kv head
-};
-
-// One sequence as the line sees it.
-struct TreeSeq {
-  int q_begin, nodes, Lk, tiles, blocks;     // blocks: of 2 * QT nodes
-  bool last_split;                           // the last block has at most QT nodes
-};
-__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int QT, int i) {
-  TreeSeq s;
-  s.q_begin = max(0, min(__ldg(p.cu_q + i), p.total_q));
-  s.nodes = max(0, min(__ldg(p.cu_q + i + 1), p.total_q) - s.q_begin);
-  s.Lk = max(0, min(__ldg(p.context_lens + i), p.bt_cols * p.block_size));
-  s.tiles = (s.Lk + kTrKv - 1) / kTrKv;
-  s.blocks = s.tiles > 0 ? (s.nodes + 2 * QT - 1) / (2 * QT) : 0;
-  s.last_split = s.nodes - (s.blocks - 1) * 2 * QT <= QT;
-  return s;
-}
-// (32 bits: the host refuses geometries whose line might be longer)
-__device__ __forceinline__ unsigned tree_cost(const TreeSeq& s, int Hkv) {
-  if (s.blocks == 0) return 0;
-  return Hkv * ((s.blocks - s.last_split) * (s.tiles * kTrTilePair + kTrUnitPair) + s.last_split * (s.tiles * kTrTileSplit + kTrUnitSplit));
-}
-// Place `off` of a sequence's part of the line: unit (block * Hkv + head) and key tile.
-__device__ __forceinline__ void tree_locate(const TreeSeq& s, int Hkv, unsigned off, int& unit, int& tile) {
-  const unsigned pair = s.tiles * kTrTilePair + kTrUnitPair;
-  const unsigned block = s.blocks == 1 ? 0 : min(off / (pair * Hkv), static_cast<unsigned>(s.blocks - 1));
-  off -= block * pair * Hkv;
-  const bool split = block == s.blocks - 1 && s.last_split;
-  const unsigned w = split ? kTrTileSplit : kTrTilePair, start = split ? kTrUnitSplit : kTrUnitPair;
-  const unsigned one = s.tiles * w + start;
-  const unsigned h = off / one;
-  off -= h * one;
-  unit = static_cast<int>(block * Hkv + h);
-  tile = static_cast<int>(off < start ? 0 : (off - start) / w);
-}
-
 // A key tile of K or V into its place: in one box per half of the dims; of a sequence's last tile only what it has (`left` keys), in
 // boxes of 16 rows.
 __device__ __forceinline__ void tree_load(const CUtensorMap* whole, const CUtensorMap* map16, uint64_t* full, unsigned char* dst, int h, int row,
@@ -130,29 +86,6 @@ __device__ __forceinline__ void tree_load(const CUtensorMap* whole, const CUtens
     tma_load_3d(dst + kTrSub + b * 2048, map16, full, 64, h, row + b * 16);
   }
 }
-// Walks along a sequence's key tiles: the cache row of each, far below zero (TMA reads zeros there) where its block is none of
-// the cache.
-struct TreeRows {
-  const int* blocks;
-  int row, in_block;
-  __device__ __forceinline__ void start(const TreeParams& p, int seq, int tile) {
-    const int col = tile * kTrKv / p.block_size;
-    blocks = p.block_tables + seq * p.bt_row_stride + col;
-    in_block = -(tile * kTrKv - col * p.block_size);        // (not looked up yet)
-  }
-  __device__ __forceinline__ int next(const TreeParams& p) {
-    if (in_block <= 0) {
-      const int blk = __ldg(blocks++);
-      row = blk >= 0 && blk < p.num_blocks ? blk * p.block_size - in_block : -(1 << 30);
-      in_block += p.block_size;
-    }
-    const int r = row;
-    row += kTrKv;
-    in_block -= kTrKv;
-    return r;
-  }
-};
-
 __device__ __forceinline__ void tree_cluster_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -228,7 +161,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
 #pragma unroll 1
     for (int i = 1; i < p.batch; ++i)
       if (max(0, min(__ldg(p.cu_q + i), p.total_q)) / (2 * QT) + i <= slot) seq = i;
-    const TreeSeq s = tree_seq(p, QT, seq);
+    const TreeSeq s = tree_seq<TcLine>(p, 2 * QT, seq);
     const int block = slot - (s.q_begin / (2 * QT) + seq), node0 = block * 2 * QT;
     c_nodes = block >= 0 ? min(s.nodes - node0, 2 * QT) : 0;
     c_row = s.q_begin + node0;
@@ -241,62 +174,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       s_at[1][2] = c_tiles * (c_rank + 1) / kTrCluster;
     }
   } else
-  // The CTA's share of the line.  (Lengths ahead of the wait below: no kernel that lets this one start early writes them.)
-  // With up to a block of sequences one sum over them gives the total and every sequence's place; larger batches take two.
-  {
-    unsigned total = 0;
-    TreeSeq s = {};
-    const int rounds = (p.batch + kTrThreads - 1) / kTrThreads;
-#pragma unroll 1
-    for (int pass = rounds > 1 ? 0 : 1; pass < 2; ++pass) {
-      unsigned upto = 0;
-#pragma unroll 1
-      for (int r = 0; r < rounds; ++r) {
-        const int i = r * kTrThreads + tid;
-        unsigned mine = 0;
-        if (i < p.batch) {
-          s = tree_seq(p, QT, i);
-          mine = tree_cost(s, p.Hkv);
-          if (s.nodes > 0 && s.tiles == 0) s_bare = 1;
-        }
-        unsigned x = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
-          if (lane >= o) x += y;
-        }
-        if (lane == 31) s_scan[warp] = x;
-        __syncthreads();
-        unsigned w = lane < kTrThreads / 32 ? s_scan[lane] : 0;
-#pragma unroll
-        for (int o = 1; o < kTrThreads / 32; o <<= 1) {
-          const unsigned y = __shfl_up_sync(0xffffffffu, w, o);
-          if (lane >= o) w += y;
-        }
-        const unsigned all = __shfl_sync(0xffffffffu, w, kTrThreads / 32 - 1), front = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-        const unsigned before = upto + (warp ? front : 0) + x - mine;
-        upto += all;
-        if (rounds == 1) total = upto;
-        else __syncthreads();
-        if (pass == 1 && mine > 0) {
-          // (any function of the CTA that grows from 0 to the total will do)
-          const unsigned one = 0xffffffffu / gridDim.x;
-#pragma unroll 1
-          for (int e = 0; e < 2; ++e) {
-            const unsigned at = __umulhi(total, one * (blockIdx.x + e));
-            if (at >= before && at < before + mine && blockIdx.x + e < gridDim.x) {
-              int unit, tile;
-              tree_locate(s, p.Hkv, at - before, unit, tile);
-              s_at[e][0] = i;
-              s_at[e][1] = unit;
-              s_at[e][2] = tile;
-            }
-          }
-        }
-      }
-      total = upto;
-    }
-  }
+    tree_share<TcLine, kTrThreads>(p, 2 * QT, s_scan, s_at, &s_bare);
   __syncthreads();
   volatile int* abort_flag = &s_abort;
   uint32_t tmem = 0;
@@ -310,7 +188,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       // sequences with nodes and no keys: zeros
 #pragma unroll 1
       for (int i = blockIdx.x; i < p.batch; i += gridDim.x) {
-        const TreeSeq s = tree_seq(p, QT, i);
+        const TreeSeq s = tree_seq<TcLine>(p, 2 * QT, i);
         if (s.tiles > 0) continue;
         uint4* const dst = reinterpret_cast<uint4*>(p.out + static_cast<long long>(s.q_begin) * p.H * 128);
         for (long long e = tid - 32; e < static_cast<long long>(s.nodes) * p.H * 16; e += kTrThreads - 32) dst[e] = make_uint4(0, 0, 0, 0);
@@ -337,7 +215,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       int2 head_unit = make_int2(0, 0);
       int seq = s_at[0][0], unit = s_at[0][1], from = s_at[0][2], have = -1;
       TreeSeq s = {};
-      TreeRows rows = {};
+      TreeRows<TcLine> rows = {};
       const int end_seq = s_at[1][0], end_unit = s_at[1][1], end_tile = s_at[1][2];
       int n_pub = 0, q_use = 0, turn = 0, k_at = 0, k_ph = 1;
       bool ok = true, started = false;
@@ -345,7 +223,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       while (ok && seq < p.batch) {
         // the next unit that has tiles here
         if (have != seq) {
-          s = tree_seq(p, QT, seq);
+          s = tree_seq<TcLine>(p, 2 * QT, seq);
           have = seq;
         }
         if (unit >= s.blocks * p.Hkv) {
@@ -500,7 +378,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       }
     } else if (warp == 3 && lane == 0) {
       // ================================ V ================================
-      TreeRows rows = {};
+      TreeRows<TcLine> rows = {};
       int n_item = 0, v_at = 0, v_ph = 1;
       bool ok = true;
       while (ok) {
@@ -1023,6 +901,13 @@ static int tree_clusters_on_chip() {
 constexpr int64_t kTrPiecesBytes = (sizeof(TreePieces) + 255) / 256 * 256;
 static int64_t tree_workspace(int ctas) { return kTrPiecesBytes + static_cast<int64_t>(ctas) * 2 * kTrPartial * 4; }
 
+int launch_tree_join(const TreeParams& p, int ctas, cudaStream_t stream) {
+  if (ctas < 2) return kOk;
+  const cudaError_t le = launch_early(tree_join_kernel, ctas * kTrJoinCtas, kTrJoinThreads, 0, stream, p, ctas);
+  g_launches.fetch_add(1);
+  return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn join launch");
+}
+
 int read_status_tree() {
   int v = 0;
   cudaMemcpyFromSymbol(&v, g_status_tree, sizeof(int));
@@ -1092,8 +977,8 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.G = G;
   p.scale_log2 = scale * 1.4426950408889634f;
   // the longest that the line of key tiles can be (table widths are all that the host knows of the lengths)
-  const double line = static_cast<double>(num_kv_heads) * (total_q / (2 * (128 / G)) + batch) *
-                      (static_cast<double>(bt_cols) * (block_size / kTrKv) * kTrTilePair + kTrUnitPair);
+  const double blocks = total_q / (G <= 16 ? 16 / G : 2 * (128 / G)) + batch;
+  const double line = num_kv_heads * blocks * (static_cast<double>(bt_cols) * (block_size / 64) * TcLine::kTilePair + TcLine::kUnitPair);
   if (line >= 2147483648.0) return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
   const int grid = sm_count();
   if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
@@ -1119,13 +1004,21 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
     g_launches.fetch_add(1);
     return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn(cluster) launch");
   }
+  // Few nodes to a sequence: tree_small.cu, up to 12 rows on average.  Us of this kernel | that one, calls on end: 256 sequences of
+  // 100 .. 2048 tokens at 16/8 heads, 1 node 210 | 180, 4 nodes 214 | 189, 8 nodes (16 rows) 224 | 215, 12 nodes 231 | 395; 128 of
+  // 500 .. 4096 at 32/8, 4 nodes (16 rows) 219 | 211; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 78 | 74; but, with 16 rows, 20 of
+  // 300 .. 2000 at 32/8, 4 nodes 31.8 | 34.3, and 64 of 500 .. 3000 at 4/2, 2 .. 14 nodes 34.1 | 38.5.
+  if (G <= 16 && static_cast<long long>(total_q) * G <= 12LL * batch) {
+    rc = make_tokens_heads_map(&map_k, k_cache, rows, num_kv_heads, row, 64);
+    if (!rc) rc = make_tokens_heads_map(&map_v, v_cache, rows, num_kv_heads, row, 64);
+    if (!rc) rc = launch_tree_small(p, map_k, map_v, map_k16, map_v16, grid, static_cast<cudaStream_t>(stream));
+    return rc ? rc : launch_tree_join(p, grid, static_cast<cudaStream_t>(stream));
+  }
   rc = tree_configure<false>();
   if (rc) return rc;
   cudaError_t le = launch_early(tree_attn_kernel<false>, grid, kTrThreads, kTrSmem, static_cast<cudaStream_t>(stream), p, map_q, map_k, map_v, map_k16, map_v16);
   g_launches.fetch_add(1);
   rc = check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn launch");
-  if (rc || grid < 2) return rc;
-  le = launch_early(tree_join_kernel, grid * kTrJoinCtas, kTrJoinThreads, 0, static_cast<cudaStream_t>(stream), p, grid);
-  g_launches.fetch_add(1);
-  return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn join launch");
+  if (rc) return rc;
+  return launch_tree_join(p, grid, static_cast<cudaStream_t>(stream));
 }

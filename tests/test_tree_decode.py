@@ -344,6 +344,24 @@ def test_attention_long_and_many(batch, ctx, nodes, H, hkv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,hkv,most", [(16, 8, 8), (32, 8, 4), (5, 1, 3), (16, 1, 1), (3, 3, 16), (24, 2, 1), (28, 4, 2)])
+@pytest.mark.parametrize("masks", ["tree", "chain", "any"])
+def test_attention_few_nodes(H, hkv, most, masks):
+    """Batches with at most 12 rows to a sequence and kv head on average: ragged contexts, none, fewer tokens than nodes, no nodes, one tile,
+    and single trees of many blocks of rows between them."""
+    rng = random.Random(H * most)
+    ctx = [1, 2, 15, 16, 17, 63, 64, 65, 0, 127, 128, 129, 300, 700, -1, 33, 2, 1100, 64, 500] * 2
+    nodes = [rng.randint(0, most) for _ in ctx]
+    nodes[3], nodes[16], nodes[8] = most, most, most
+    nodes[13] = 3 * most + 5
+    while sum(nodes) * (H // hkv) > 12 * len(ctx):
+        nodes[nodes.index(max(nodes[14:]), 14)] -= 1
+    c = attention_case(H, hkv, ctx, nodes, seed=most, masks=masks, extra_rows=0)
+    check_attention(c, run_attention(c))
+    status_ok()
+
+
+@pytest.mark.gpu
 def test_attention_block_size_words_and_values():
     """Blocks of 512, masks with more words than nodes, large and small scores, an equal score everywhere."""
     for scale_q, bs, words in ((30.0, 512, 3), (1e-3, 256, 4), (0.0, 768, 1)):
