@@ -16,8 +16,8 @@
 // The halves are two softmax chains.  Work is a row of steps that they take in strict turn, across the units' borders: a step is a
 // key tile of a unit with at most 128 rows (the output warpgroup joins what the halves have of it), or a key tile for one of the
 // two Q tiles of a larger unit.
-// kCluster, for few units: a thread-block cluster of 8 CTAs has a unit and shares its key tiles out; their partial results are joined
-// through distributed shared memory, each CTA joining and writing 16 of the dims, so there is no second launch.
+// kCluster, for few units: a thread-block cluster of 2, 4 or 8 CTAs has a unit and shares its key tiles out; their partial results are
+// joined through distributed shared memory, each CTA joining and writing its part of the dims, so there is no second launch.
 // TMEM: S [0,128)  P_A [128,192)  P_B [192,256)  O_A [256,384)  O_B [384,512).  Both halves' scores go through one S: a row is in
 // its thread's registers 200 cycles after the product, and then the next step's product may run.  With an S of its own in
 // which P replaced the scores, a half's next S had to wait for its P V: a chain of 3740 cycles a tile at 256 rows, of which the
@@ -100,9 +100,10 @@ __device__ __forceinline__ uint32_t tree_cluster_addr(uint32_t addr, uint32_t ra
 __device__ __forceinline__ void tree_cluster_store(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
-// What the CTAs of a cluster send one another, in the room of the rings: for each of them 16 dims and then maxima and sums of 256 rows.
-constexpr int kTrCluster = 8;
-constexpr int kTrInbox = (16 + 2) * 256;      // floats of one sender
+// What the CTAs of a cluster send one another, in the room of the rings: from each of them 128 / CTAs dims, then maxima and sums,
+// of 256 rows.
+constexpr int kTrClusterMax = 8;
+static_assert(2 * (64 + 2) * 256 * 4 <= 7 * kTrTile && kTrClusterMax * (16 + 2) * 256 * 4 <= 7 * kTrTile, "inbox");
 
 template <bool kCluster>
 __global__ void __launch_bounds__(kTrThreads, 1)
@@ -152,10 +153,11 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   }
   __syncthreads();
   int c_nodes = 0, c_row = 0, c_head = 0, c_tiles = 0;       // kCluster: the cluster's unit
-  const int c_rank = blockIdx.x % kTrCluster;
+  const int c_size = kCluster ? p.cluster : 1, c_rank = blockIdx.x % c_size;         // CTAs of a cluster: 2, 4 or 8
+  const int c_dims = 128 / c_size, c_inbox = (c_dims + 2) * 256;                        // floats of one sender
   if constexpr (kCluster) {
     // sequence i owns blocks of nodes [cu_q[i] / (2 * QT) + i, ...); there are few sequences
-    const int x = static_cast<int>(blockIdx.x / kTrCluster), slot = x / p.Hkv;
+    const int x = static_cast<int>(blockIdx.x / c_size), slot = x / p.Hkv;
     c_head = x - slot * p.Hkv;
     int seq = 0;
 #pragma unroll 1
@@ -170,8 +172,8 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       s_bare = c_rank == 0 && c_tiles == 0;
       s_at[0][0] = s_at[1][0] = c_tiles > 0 ? seq : p.batch;
       s_at[0][1] = s_at[1][1] = block * p.Hkv + c_head;
-      s_at[0][2] = c_tiles * c_rank / kTrCluster;
-      s_at[1][2] = c_tiles * (c_rank + 1) / kTrCluster;
+      s_at[0][2] = c_tiles * c_rank / c_size;
+      s_at[1][2] = c_tiles * (c_rank + 1) / c_size;
     }
   } else
     tree_share<TcLine, kTrThreads>(p, 2 * QT, s_scan, s_at, &s_bare);
@@ -618,12 +620,12 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
           const int t = r / G;
           __nv_bfloat16* const dst = p.out + (static_cast<long long>(it.q_row + turn * QT + t) * p.H + it.h * G + (r - t * G)) * 128;
           float* const part = kCluster || it.partial < 0 ? nullptr : p.partials + static_cast<long long>(it.partial) * kTrPartial + (turn * 4 + quarter) * kTrGroup + lane;
-          const uint32_t inbox = smem_u32(smem) + (c_rank * kTrInbox + turn * 128 + r) * 4;
+          const uint32_t inbox = smem_u32(smem) + (c_rank * c_inbox + turn * 128 + r) * 4;
           if constexpr (kCluster) {
 #pragma unroll 1
-            for (int x = 0; x < kTrCluster; ++x) {
-              tree_cluster_store(tree_cluster_addr(inbox + 16 * 1024, x), M);
-              tree_cluster_store(tree_cluster_addr(inbox + 17 * 1024, x), sum);
+            for (int x = 0; x < c_size; ++x) {
+              tree_cluster_store(tree_cluster_addr(inbox + c_dims * 1024, x), M);
+              tree_cluster_store(tree_cluster_addr(inbox + (c_dims + 1) * 1024, x), sum);
             }
           } else if (part) {
             part[128 * 32] = M;
@@ -649,7 +651,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
 #pragma unroll
             for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), wb, __uint_as_float(a[i]) * wa));
             if constexpr (kCluster) {
-              const uint32_t to = tree_cluster_addr(inbox, cch);
+              const uint32_t to = tree_cluster_addr(inbox + (cch * 16 % c_dims) * 1024, cch * 16 / c_dims);
 #pragma unroll
               for (int i = 0; i < 16; ++i) tree_cluster_store(to + i * 1024, __uint_as_float(a[i]));
             } else if (part) {
@@ -681,31 +683,37 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   if constexpr (kCluster) {
     if (!met) tree_cluster_sync();             // (output warps that had an item have been here before)
     tree_cluster_sync();
-    // all partial results are here: a thread joins 8 of this CTA's 16 dims of a row
+    // all partial results are here: a thread joins a row, 8 of this CTA's dims at a time
     const float* const inbox = reinterpret_cast<const float*>(smem);
     const int row = tid & 255, half = row >> 7, r = row & 127, t = r / G, node = half * QT + t;
     if (r < QT * G && node < c_nodes && c_tiles > 0) {
+      // (with fewer tiles than CTAs some have sent nothing)
       float M = -INFINITY;
 #pragma unroll 1
-      for (int x = 0; x < kTrCluster; ++x)
-        if (c_tiles * (x + 1) / kTrCluster > c_tiles * x / kTrCluster) M = fmaxf(M, inbox[x * kTrInbox + 16 * 256 + row]);
+      for (int x = 0; x < c_size; ++x)
+        if (c_tiles * (x + 1) / c_size > c_tiles * x / c_size) M = fmaxf(M, inbox[x * c_inbox + c_dims * 256 + row]);
       const float ref = M == -INFINITY ? 0.f : M;
-      float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      __nv_bfloat16* const dst = p.out + (static_cast<long long>(c_row + node) * p.H + c_head * G + (r - t * G)) * 128 + c_rank * c_dims;
 #pragma unroll 1
-      for (int x = 0; x < kTrCluster; ++x) {
-        if (c_tiles * (x + 1) / kTrCluster == c_tiles * x / kTrCluster) continue;
-        const float w = fast_exp2(inbox[x * kTrInbox + 16 * 256 + row] - ref);
-        sum = fmaf(inbox[x * kTrInbox + 17 * 256 + row], w, sum);
+      for (int d = (tid >> 8) * 8; d < c_dims; d += 16) {
+        float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int x = 0; x < c_size; ++x) {
+          if (c_tiles * (x + 1) / c_size == c_tiles * x / c_size) continue;
+          const float* const from = inbox + x * c_inbox + row;
+          const float w = fast_exp2(from[c_dims * 256] - ref);
+          sum = fmaf(from[(c_dims + 1) * 256], w, sum);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = fmaf(inbox[x * kTrInbox + ((tid >> 8) * 8 + i) * 256 + row], w, o[i]);
+          for (int i = 0; i < 8; ++i) o[i] = fmaf(from[(d + i) * 256], w, o[i]);
+        }
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        uint4 v;
+        v.x = pack_bf16(o[0] * inv, o[1] * inv);
+        v.y = pack_bf16(o[2] * inv, o[3] * inv);
+        v.z = pack_bf16(o[4] * inv, o[5] * inv);
+        v.w = pack_bf16(o[6] * inv, o[7] * inv);
+        *reinterpret_cast<uint4*>(dst + d) = v;
       }
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      uint4 v;
-      v.x = pack_bf16(o[0] * inv, o[1] * inv);
-      v.y = pack_bf16(o[2] * inv, o[3] * inv);
-      v.z = pack_bf16(o[4] * inv, o[5] * inv);
-      v.w = pack_bf16(o[6] * inv, o[7] * inv);
-      reinterpret_cast<uint4*>(p.out + (static_cast<long long>(c_row + node) * p.H + c_head * G + (r - t * G)) * 128)[c_rank * 2 + (tid >> 8)] = v;
     }
   }
   // ---- teardown: everyone meets, then the allocating warp frees TMEM ----
@@ -857,43 +865,49 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
 }
 
 constexpr size_t kTrSmem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTile;
-// Table width (in key tiles) up to which few units go to clusters.
-constexpr int kTrClusterTiles = 64;
+// Sizes of clusters, and how wide (in key tiles) the table may be for each: what the host knows of the lengths.  Us with the join |
+// with clusters, calls on end:
+//   8   1 sequence of 300, 4000, 12000 tokens, 9 nodes, 16/8 heads   14.0, 18.3, 23.1 | 9.6, 12.2, 18.8; 60 nodes, 8/2 heads
+//       16.3, 22.4, 32.4 | 13.2, 20.3, 31.6, and of 16000 32.5 | 37.5
+//   4   4 of 500, 2000, 4000, 20 nodes, 32/8   18.6, 21.9, 28.1 | 11.2, 16.5, 24.8; of 200 .. 4000, 300 .. 8000   21.4, 28.1 | 22.7, 36.3
+//   2   9 of 500, 2000, 4000, 9 nodes, 16/8    17.2, 26.4, 38.2 | 14.0, 22.0, 32.8; 6 of 200 .. 4000, 300 .. 8000   24.1, 32.1 | 23.4, 37.2
+constexpr int kTrClusterSizes = 3;
+constexpr int kTrClusterTiles[kTrClusterSizes] = {128, 40, 32};
 
 template <bool kCluster>
 static int tree_configure() {
   static std::atomic<size_t> configured[kMaxDevices];
   return ensure_dynamic_smem(reinterpret_cast<const void*>(tree_attn_kernel<kCluster>), kTrSmem, configured, "tree_attn: cudaFuncSetAttribute");
 }
-static void tree_cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, unsigned clusters, cudaStream_t stream) {
-  cfg->gridDim = dim3(clusters * kTrCluster);
+static void tree_cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attr, unsigned clusters, unsigned size, cudaStream_t stream) {
+  cfg->gridDim = dim3(clusters * size);
   cfg->blockDim = dim3(kTrThreads);
   cfg->dynamicSmemBytes = kTrSmem;
   cfg->stream = stream;
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kTrCluster;
+  attr[0].val.clusterDim.x = size;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg->attrs = attr;
   cfg->numAttrs = 2;
 }
-// How many clusters the current device holds at a time (0: not known).
-static int tree_clusters_on_chip() {
-  static std::atomic<int> known[kMaxDevices];
+// How many clusters of 8 >> i CTAs the current device holds at a time (0: not known).
+static int tree_clusters_on_chip(int i) {
+  static std::atomic<int> known[kMaxDevices][kTrClusterSizes];
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
-  if ((n = known[dev].load(std::memory_order_acquire)) > 0) return n;
+  if ((n = known[dev][i].load(std::memory_order_acquire)) > 0) return n;
   if (tree_configure<true>()) return 0;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  tree_cluster_config(&cfg, attr, 1, nullptr);
+  tree_cluster_config(&cfg, attr, 1, kTrClusterMax >> i, nullptr);
   cfg.numAttrs = 1;
   if (cudaOccupancyMaxActiveClusters(&n, tree_attn_kernel<true>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
-  known[dev].store(n, std::memory_order_release);
+  known[dev][i].store(n, std::memory_order_release);
   return n;
 }
 
@@ -994,12 +1008,14 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   if (rc) return rc;
   // few units: a cluster each, one launch
   const long long units = (static_cast<long long>(total_q) / (2 * (128 / G)) + batch) * num_kv_heads;
-  if (static_cast<long long>(bt_cols) * (block_size / kTrKv) <= kTrClusterTiles && units <= tree_clusters_on_chip()) {
+  for (int i = 0; i < kTrClusterSizes; ++i) {
+    if (static_cast<long long>(bt_cols) * (block_size / kTrKv) > kTrClusterTiles[i] || units > tree_clusters_on_chip(i)) continue;
     rc = tree_configure<true>();
     if (rc) return rc;
+    p.cluster = kTrClusterMax >> i;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    tree_cluster_config(&cfg, attr, static_cast<unsigned>(units), static_cast<cudaStream_t>(stream));
+    tree_cluster_config(&cfg, attr, static_cast<unsigned>(units), static_cast<unsigned>(p.cluster), static_cast<cudaStream_t>(stream));
     const cudaError_t le = cudaLaunchKernelEx(&cfg, tree_attn_kernel<true>, p, map_q, map_k, map_v, map_k16, map_v16);
     g_launches.fetch_add(1);
     return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn(cluster) launch");
