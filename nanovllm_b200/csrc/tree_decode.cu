@@ -31,6 +31,7 @@ __global__ void __launch_bounds__(kAcceptWarps * 32) accept_tree_kernel(const Ac
   const int cached = p.cached[i];
   int count = 0;
   if (p.context[i] > 0 && nodes > 0) {
+#pragma unroll 4
     for (int n = lane; n < min(nodes, kAcceptNodes); n += 32) {
       s_draft[warp][n] = p.draft[start + n];
       s_target[warp][n] = p.target[start + n];
@@ -75,15 +76,15 @@ __global__ void __launch_bounds__(kAcceptWarps * 32) accept_tree_kernel(const Ac
 // ---- the cache ------------------------------------------------------------------------------------------------------
 // Row start + path[k] of every plane goes to start + k.  Entries below their place (path[k] < k) are not moved, so a row that is
 // written (k) is read by later moves only where path[k'] = k < k', which that excludes: a thread may have the loads of
-// several moves in flight, and keeps to one 16-byte column of a row.
+// several moves in flight, and keeps to one 16-byte column of a row.  A few MB at most move, so what counts is the way there: lengths
+// and path, then the table, then the rows, a round trip each.  Every warp goes it by itself, a move to a lane.
 constexpr int kCompactThreads = 256;
-constexpr int kCompactPath = 256;        // entries of a path that are looked at together
 
 struct CompactParams {
   char* cache;
   long long plane_stride, row_bytes;
-  int planes, vecs;                      // vecs: 16-byte columns of a row
-  long long columns;                     // planes * vecs
+  unsigned vecs;                         // 16-byte columns of a row
+  unsigned columns;                      // of all planes
   int num_blocks, block_size;
   const int *path, *accepted, *start, *block_tables;
   int path_cols;
@@ -99,54 +100,41 @@ __device__ __forceinline__ long long compact_row(const CompactParams& p, const i
 }
 
 __global__ void __launch_bounds__(kCompactThreads) compact_kvcache_kernel(const CompactParams p) {
-  __shared__ long long s_src[kCompactPath], s_dst[kCompactPath];
-  __shared__ int s_moves;
-  const int i = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int i = blockIdx.y, lane = threadIdx.x & 31;
   const int* const table = p.block_tables + i * p.bt_row_stride;
-  const long long column = static_cast<long long>(blockIdx.x) * kCompactThreads + tid;
-  char* mine = nullptr;
-  if (column < p.columns) {
-    const long long plane = column / p.vecs;
-    mine = p.cache + plane * p.plane_stride + (column - plane * p.vecs) * 16;
-  }
-  const int n = min(p.accepted[i], p.path_cols), start = p.start[i];
-  for (int base = 0; base < n; base += kCompactPath) {
-    if (tid < 32) {
-      int moves = 0;
-      for (int k0 = base; k0 < min(n, base + kCompactPath); k0 += 32) {
-        const int k = k0 + lane;
-        long long src = -1, dst = -1;
-        if (k < n) {
-          const int node = p.path[static_cast<long long>(i) * p.path_cols + k];
-          if (node > k && node <= 0x7fffffff - start) {
-            src = compact_row(p, table, start + node);
-            dst = compact_row(p, table, start + k);
-          }
-        }
-        const bool move = src >= 0 && dst >= 0;
-        const unsigned all = __ballot_sync(0xffffffffu, move);
-        if (move) {
-          const int at = moves + __popc(all & ((1u << lane) - 1));
-          s_src[at] = src * p.row_bytes;
-          s_dst[at] = dst * p.row_bytes;
-        }
-        moves += __popc(all);
-      }
-      if (lane == 0) s_moves = moves;
+  const int* const path = p.path + static_cast<long long>(i) * p.path_cols;
+  int node = lane < p.path_cols ? path[lane] : -1;
+  const int start = p.start[i], n = min(p.accepted[i], p.path_cols);
+  const unsigned column = blockIdx.x * kCompactThreads + threadIdx.x;
+  const bool live = column < p.columns;
+  const unsigned plane = column / p.vecs;
+  char* const mine = p.cache + plane * p.plane_stride + (column - plane * p.vecs) * 16;
+  for (int base = 0; base < n; base += 32) {
+    const int k = base + lane;
+    if (base > 0) node = k < n ? path[k] : -1;
+    long long src = -1, dst = -1;
+    if (k < n && node > k && node <= 0x7fffffff - start) {
+      src = compact_row(p, table, start + node);
+      dst = compact_row(p, table, start + k);
     }
-    __syncthreads();
-    const int moves = s_moves;
-    if (mine)
-      for (int k = 0; k < moves; k += 8) {
-        uint4 v[8];
+    unsigned moves = __ballot_sync(0xffffffffu, src >= 0 && dst >= 0);
+    src *= p.row_bytes;
+    dst *= p.row_bytes;
+    while (moves) {
+      uint4 v[8];
+      long long to[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (k + u < moves) v[u] = *reinterpret_cast<const uint4*>(mine + s_src[k + u]);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (k + u < moves) *reinterpret_cast<uint4*>(mine + s_dst[k + u]) = v[u];
+      for (int u = 0; u < 8; ++u) {
+        const int from = __ffs(moves) - 1;             // (-1: none left)
+        moves &= moves - 1;
+        const long long at = __shfl_sync(0xffffffffu, src, from & 31);
+        to[u] = from >= 0 ? __shfl_sync(0xffffffffu, dst, from & 31) : -1;
+        if (live && from >= 0) v[u] = *reinterpret_cast<const uint4*>(mine + at);
       }
-    __syncthreads();
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (live && to[u] >= 0) *reinterpret_cast<uint4*>(mine + to[u]) = v[u];
+    }
   }
 }
 
@@ -195,13 +183,14 @@ extern "C" int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_s
   if (bt_cols <= 0 || bt_row_stride < bt_cols) return set_error(kErrBadShape, "compact_kvcache: bad block table geometry");
   if (row_bytes <= 0 || row_bytes > (1 << 20) || plane_stride_bytes < num_blocks * block_size * row_bytes) return set_error(kErrBadShape, "compact_kvcache: rows of 1 to 2^20 bytes, planes that do not overlap");
   if ((reinterpret_cast<uintptr_t>(cache) | row_bytes | plane_stride_bytes) & 15) return set_error(kErrMisaligned, "compact_kvcache: cache, rows and planes must be multiples of 16 bytes");
+  const long long columns = planes * (row_bytes / 16);
+  if (columns >= 0x7fffffffLL) return set_error(kErrBadShape, "compact_kvcache: too many planes");
   CompactParams p;
   p.cache = static_cast<char*>(cache);
   p.plane_stride = plane_stride_bytes;
   p.row_bytes = row_bytes;
-  p.planes = planes;
-  p.vecs = static_cast<int>(row_bytes / 16);
-  p.columns = static_cast<long long>(planes) * p.vecs;
+  p.vecs = static_cast<unsigned>(row_bytes / 16);
+  p.columns = static_cast<unsigned>(columns);
   p.num_blocks = static_cast<int>(num_blocks);
   p.block_size = block_size;
   p.path = path;
@@ -211,9 +200,8 @@ extern "C" int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_s
   p.path_cols = path_cols;
   p.bt_row_stride = bt_row_stride;
   p.bt_cols = bt_cols;
-  const long long blocks = (p.columns + kCompactThreads - 1) / kCompactThreads;
-  if (blocks > 0x7fffffffLL) return set_error(kErrBadShape, "compact_kvcache: too many planes");
-  compact_kvcache_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch)), kCompactThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const unsigned blocks = (p.columns + kCompactThreads - 1) / kCompactThreads;
+  compact_kvcache_kernel<<<dim3(blocks, static_cast<unsigned>(batch)), kCompactThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   g_launches.fetch_add(1);
   return check_cuda(cudaGetLastError(), "compact_kvcache launch");
 }
