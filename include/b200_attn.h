@@ -20,14 +20,17 @@
  *    >= ceil(len / block_size) may hold -1 or stale ids (nanovllm/engine/model_runner.py:119-123,
  *    :203) and are never dereferenced.
  *  - Early starts (programmatic dependent launch).  b200_store_kvcache, b200_qk_norm_rope_store, b200_decode_attn,
- *    b200_store_decode_attn and b200_prefill_attn / b200_store_prefill_attn start early behind a kernel that lets its
- *    dependents do so (griddepcontrol.launch_dependents), and read part of their metadata before they wait for it:
+ *    b200_store_decode_attn, b200_prefill_attn / b200_store_prefill_attn, b200_tree_attn and the other entry points for
+ *    steps with drafted tokens start early behind a kernel that lets its dependents do so (griddepcontrol.launch_dependents), and read part of their metadata before they wait for it:
  *      decode                 context_lens, block_tables; b200_store_decode_attn also slot_mapping
  *      prefill, tcgen05       cu_seqlens_q, cu_seqlens_k
+ *      tree attention         cu_seqlens_q, context_lens, block_tables
  *      store, producer, prefill on mma.sync     nothing (what the first two read ahead they read again)
+ *      step tables, release, accept, compaction     nothing
  *    So a kernel that lets its dependents start early must not write these arrays.  Of this library the store,
- *    producer, decode and mma.sync prefill kernels do (they write cache rows, q, k and outputs only); the metadata unpack,
- *    all-reduce and tcgen05 prefill kernels do not.  Behind any other kernel or copy there is nothing to observe.
+ *    producer, decode, tree attention and mma.sync prefill kernels do (they write cache rows, q, k, outputs and workspaces
+ *    only); the metadata unpack, all-reduce and tcgen05 prefill kernels, and the step's tables, release, accept and
+ *    compaction, which write such arrays, do not.  Behind any other kernel or copy there is nothing to observe.
  *  - Return value: 0 on success; negative = arguments rejected before any launch; positive = a
  *    cudaError_t from the launch.  b200_last_error() describes the last failure of the calling
  *    thread.  Nothing throws, aborts or traps.

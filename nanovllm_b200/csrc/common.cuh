@@ -49,10 +49,10 @@ int make_tokens_heads_map_cols32(CUtensorMap* map, const void* base, uint64_t to
 // Launch with programmatic stream serialization: the kernel may start while the one in front of it in the stream still
 // runs, if that one lets it (griddepcontrol.launch_dependents), and waits for it itself (griddepcontrol.wait).
 template <typename... Params, typename... Args>
-inline cudaError_t launch_early(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
+inline cudaError_t launch_early(void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
                                 Args... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;

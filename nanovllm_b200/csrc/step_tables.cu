@@ -71,13 +71,16 @@ __device__ __forceinline__ StepSum block_scan(StepSum v, StepSum* scratch /* [kS
 }
 
 // Marks, for each row that occurs in rows[0 .. batch), its first place: open addressing with as many slots as twice the batch.
-__device__ __forceinline__ void hash_rows(const int* rows, int batch, int hash_slots, int* keys, int* firsts) {
-  for (int i = threadIdx.x; i < hash_slots; i += blockDim.x) {
+// (The table has been cleared.)
+__device__ __forceinline__ void hash_clear(int hash_slots, int* keys, int* firsts) {
+  for (int i = threadIdx.x; i < hash_slots; i += kStepThreads) {
     keys[i] = INT_MIN;
     firsts[i] = INT_MAX;
   }
+}
+__device__ __forceinline__ void hash_rows(const int* rows, int batch, int hash_slots, int* keys, int* firsts) {
   __syncthreads();
-  for (int i = threadIdx.x; i < batch; i += blockDim.x) {
+  for (int i = threadIdx.x; i < batch; i += kStepThreads) {
     const int r = rows[i];
     if (r < 0) continue;
     for (unsigned s = static_cast<unsigned>(r) * 2654435761u >> 7;; ++s) {
@@ -111,6 +114,9 @@ __global__ void __cluster_dims__(kStepCtas, 1, 1) __launch_bounds__(kStepThreads
   __shared__ StepSum scratch[2][kStepThreads / 32];
   __shared__ int s_granted;
   const int tid = threadIdx.x, rank = blockIdx.x;
+  hash_clear(p.hash_slots, s_keys, s_firsts);
+  if (tid == 0) s_granted = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");     // from here on: what the kernel in front may have written
   // What stands in the way is one load behind the other, so the first ones go out together: the thread's sequence, and the
   // parents of its tokens on their way into L1.
   const int n_free = max(0, min(p.pool[0], p.num_blocks));
@@ -120,7 +126,6 @@ __global__ void __cluster_dims__(kStepCtas, 1, 1) __launch_bounds__(kStepThreads
     for (int t = rank * kStepThreads + tid; t < p.num_tokens; t += kStepCtas * kStepThreads)
       asm volatile("prefetch.global.L1 [%0];" ::"l"(p.parents + t));
   const int owned0 = row0 >= 0 && row0 < p.max_requests ? p.owned[row0] : 0;
-  if (tid == 0) s_granted = 0;
   if (p.rows) hash_rows(p.rows, p.batch, p.hash_slots, s_keys, s_firsts);
   else __syncthreads();
   long long tokens = 0, keys_so_far = 0;
@@ -268,6 +273,8 @@ __global__ void __launch_bounds__(kStepThreads, 1) release_blocks_kernel(const R
   int* const s_firsts = s_keys + p.hash_slots;
   __shared__ StepSum scratch[kStepThreads / 32];
   const int tid = threadIdx.x;
+  hash_clear(p.hash_slots, s_keys, s_firsts);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int n_free = max(0, min(p.pool[0], p.num_blocks));
   const bool live0 = tid < p.batch;
   const int row0 = live0 ? (p.rows ? p.rows[tid] : tid) : -1, len0 = live0 ? p.keep_lens[tid] : 0;
@@ -382,9 +389,9 @@ extern "C" int b200_step_tables(const int32_t* rows, const int32_t* cached_lens,
     rc = ensure_dynamic_smem(reinterpret_cast<const void*>(step_tables_kernel), smem, configured, "step_tables: cudaFuncSetAttribute");
     if (rc) return rc;
   }
-  step_tables_kernel<<<kStepCtas, kStepThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaError_t le = launch_early(step_tables_kernel, kStepCtas, kStepThreads, smem, static_cast<cudaStream_t>(stream), p);
   g_launches.fetch_add(1);
-  return check_cuda(cudaGetLastError(), "step_tables launch");
+  return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "step_tables launch");
 }
 
 extern "C" int b200_release_blocks(const int32_t* rows, const int32_t* keep_lens, int32_t batch, int32_t block_size, int32_t* tables,
@@ -415,7 +422,7 @@ extern "C" int b200_release_blocks(const int32_t* rows, const int32_t* keep_lens
     rc = ensure_dynamic_smem(reinterpret_cast<const void*>(release_blocks_kernel), smem, configured, "release_blocks: cudaFuncSetAttribute");
     if (rc) return rc;
   }
-  release_blocks_kernel<<<1, kStepThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaError_t le = launch_early(release_blocks_kernel, 1, kStepThreads, smem, static_cast<cudaStream_t>(stream), p);
   g_launches.fetch_add(1);
-  return check_cuda(cudaGetLastError(), "release_blocks launch");
+  return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "release_blocks launch");
 }

@@ -27,6 +27,7 @@ __global__ void __launch_bounds__(kAcceptWarps * 32) accept_tree_kernel(const Ac
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int i = blockIdx.x * kAcceptWarps + warp;
   if (i >= p.batch) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int start = max(0, min(p.cu[i], p.num_tokens)), nodes = max(0, min(p.cu[i + 1], p.num_tokens) - start);
   const int cached = p.cached[i];
   int count = 0;
@@ -101,6 +102,7 @@ __device__ __forceinline__ long long compact_row(const CompactParams& p, const i
 
 __global__ void __launch_bounds__(kCompactThreads) compact_kvcache_kernel(const CompactParams p) {
   const int i = blockIdx.y, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int* const table = p.block_tables + i * p.bt_row_stride;
   const int* const path = p.path + static_cast<long long>(i) * p.path_cols;
   int node = lane < p.path_cols ? path[lane] : -1;
@@ -113,7 +115,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_kvcache_kernel(const 
     const int k = base + lane;
     if (base > 0) node = k < n ? path[k] : -1;
     long long src = -1, dst = -1;
-    if (k < n && node > k && node <= 0x7fffffff - start) {
+    if (k < n && start >= 0 && node > k && node <= 0x7fffffff - start) {
       src = compact_row(p, table, start + node);
       dst = compact_row(p, table, start + k);
     }
@@ -166,9 +168,10 @@ extern "C" int b200_accept_tree(const int64_t* draft_tokens, const int64_t* targ
   p.path = path;
   p.cached_out = new_cached_lens;
   p.tokens = reinterpret_cast<long long*>(tokens);
-  accept_tree_kernel<<<(batch + kAcceptWarps - 1) / kAcceptWarps, kAcceptWarps * 32, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaError_t le = launch_early(accept_tree_kernel, (static_cast<unsigned>(batch) + kAcceptWarps - 1) / kAcceptWarps, kAcceptWarps * 32, 0,
+                                      static_cast<cudaStream_t>(stream), p);
   g_launches.fetch_add(1);
-  return check_cuda(cudaGetLastError(), "accept_tree launch");
+  return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "accept_tree launch");
 }
 
 extern "C" int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_stride_bytes, int64_t row_bytes, int64_t num_blocks,
@@ -201,7 +204,8 @@ extern "C" int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_s
   p.bt_row_stride = bt_row_stride;
   p.bt_cols = bt_cols;
   const unsigned blocks = (p.columns + kCompactThreads - 1) / kCompactThreads;
-  compact_kvcache_kernel<<<dim3(blocks, static_cast<unsigned>(batch)), kCompactThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaError_t le = launch_early(compact_kvcache_kernel, dim3(blocks, static_cast<unsigned>(batch)), kCompactThreads, 0,
+                                      static_cast<cudaStream_t>(stream), p);
   g_launches.fetch_add(1);
-  return check_cuda(cudaGetLastError(), "compact_kvcache launch");
+  return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "compact_kvcache launch");
 }
