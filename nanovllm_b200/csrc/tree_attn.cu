@@ -289,9 +289,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       }
       if (!started) asm volatile("griddepcontrol.wait;" ::: "memory");
       if constexpr (!kCluster) {
-        p.pieces->cont[blockIdx.x] = cont;
-        p.pieces->head[blockIdx.x] = head;
-        p.pieces->unit[blockIdx.x] = head_unit;
+        p.pieces->of[blockIdx.x] = make_int4(head, cont, head_unit.x, head_unit.y);
       }
       if (ok) {
         const int is = n_pub % kTrItems;
@@ -749,26 +747,23 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
     mbar_init(&s_bar, 1);
     mbar_fence_init();
   }
+  int loads = 0;                              // phases of the barrier
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int head[kTrJoinWords], cont[kTrJoinWords];
-  int2 unit_of[kTrJoinWords];
+  int4 piece[kTrJoinWords];                   // nodes of the unit that begins (0: none), how the share begins, that unit
 #pragma unroll
   for (int w = 0; w < kTrJoinWords; ++w) {
     const int c = w * 32 + lane;
-    head[w] = c < ctas ? __ldcg(p.pieces->head + c) : 0;
-    cont[w] = c < ctas ? __ldcg(p.pieces->cont + c) : 0;
-    unit_of[w] = c < ctas ? __ldcg(p.pieces->unit + c) : make_int2(0, 0);
+    piece[w] = c < ctas ? p.pieces->of[c] : make_int4(0, 0, 0, 0);
   }
   unsigned heads[kTrJoinWords];
   int units = 0;
 #pragma unroll
   for (int w = 0; w < kTrJoinWords; ++w) {
-    heads[w] = __ballot_sync(0xffffffffu, head[w] > 0);
+    heads[w] = __ballot_sync(0xffffffffu, piece[w].x > 0);
     units += __popc(heads[w]);
   }
   // tasks of a unit: 8 groups x 1, 2, 4 or 8 slices of the dims, so that there are about as many as CTAs
-  const int shift = units > 74 ? 0 : units > 37 ? 1 : units > 18 ? 2 : 3;
-  int loads = 0;                              // phases of the barrier
+  const int shift = units > 111 ? 0 : units > 55 ? 1 : units > 27 ? 2 : 3;
 #pragma unroll 1
   for (int task = blockIdx.x; task < units << (3 + shift); task += gridDim.x) {
     // the unit: the CTA that has its first piece, and how many nodes
@@ -776,12 +771,12 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
     int2 unit = make_int2(0, 0);
 #pragma unroll
     for (int w = 0; w < kTrJoinWords; ++w) {
-      const unsigned found = __ballot_sync(0xffffffffu, head[w] > 0 && __popc(heads[w] & ((1u << lane) - 1)) == k);
+      const unsigned found = __ballot_sync(0xffffffffu, piece[w].x > 0 && __popc(heads[w] & ((1u << lane) - 1)) == k);
       if (found) {
         c0 = w * 32 + __ffs(found) - 1;
-        nodes_all = __shfl_sync(0xffffffffu, head[w], __ffs(found) - 1);
-        unit.x = __shfl_sync(0xffffffffu, unit_of[w].x, __ffs(found) - 1);
-        unit.y = __shfl_sync(0xffffffffu, unit_of[w].y, __ffs(found) - 1);
+        nodes_all = __shfl_sync(0xffffffffu, piece[w].x, __ffs(found) - 1);
+        unit.x = __shfl_sync(0xffffffffu, piece[w].z, __ffs(found) - 1);
+        unit.y = __shfl_sync(0xffffffffu, piece[w].w, __ffs(found) - 1);
       }
       k -= __popc(heads[w]);
     }
@@ -796,8 +791,8 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
 #pragma unroll
     for (int w = 0; w < kTrJoinWords; ++w) {
       const int c = w * 32 + lane;
-      const unsigned after = __ballot_sync(0xffffffffu, c > c0), last = __ballot_sync(0xffffffffu, cont[w] == 2) & after;
-      unsigned mine = __ballot_sync(0xffffffffu, cont[w] != 0) & after;
+      const unsigned after = __ballot_sync(0xffffffffu, c > c0), last = __ballot_sync(0xffffffffu, piece[w].y == 2) & after;
+      unsigned mine = __ballot_sync(0xffffffffu, piece[w].y != 0) & after;
       if (last) mine &= last ^ (last - 1);    // up to the first of them
       if (!open) mine = 0;
       if (warp == 0 && (mine >> lane) & 1) s_list[n + __popc(mine & ((1u << lane) - 1))] = static_cast<short>(2 * c);
@@ -812,7 +807,7 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
     const int dims = min(dims_all, n <= 2 ? 128 : n <= 4 ? 64 : n <= 8 ? 32 : 16), stride = dims * 32 + 64;
 #pragma unroll 1
     for (int dim0 = first_dim; dim0 < first_dim + dims_all; dim0 += dims) {
-      float M = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+      float M = -INFINITY, sum = 0.f, o[16];
 #pragma unroll 1
       for (int base = 0; base < n; base += kTrJoinPieces) {
         const int m = min(n - base, kTrJoinPieces);
@@ -832,12 +827,12 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
         ++loads;
         // every warp for itself: the new maximum and sum; the weights are shared out
         float top = M;
-#pragma unroll 1
+#pragma unroll 4
         for (int x = 0; x < m; ++x) top = fmaxf(top, s_buf[x * stride + dims * 32 + lane]);
         const float ref = top == -INFINITY ? 0.f : top, was = fast_exp2(M - ref);
         M = top;
         sum *= was;
-#pragma unroll 1
+#pragma unroll 4
         for (int x = 0; x < m; ++x) {
           const float w = fast_exp2(s_buf[x * stride + dims * 32 + lane] - ref);
           sum = fmaf(s_buf[x * stride + dims * 32 + 32 + lane], w, sum);
@@ -845,20 +840,36 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
         }
         __syncthreads();
         const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        // 4 dims of a warp at a time (more pieces follow with 16 dims only, which is once)
+        // a row's dims are a quarter to each warp, up to 16 at a time: two stores then fill a sector (more pieces follow with
+        // 16 dims only)
+        const auto join = [&](auto width) {
+          constexpr int N = decltype(width)::value;
 #pragma unroll 1
-        for (int d = warp * 4; d < dims; d += 16) {
+          for (int d = warp * N; d < dims; d += 4 * N) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = base ? o[i] * was : 0.f;
+            for (int i = 0; i < N; ++i) o[i] = N == 4 && base ? o[i] * was : 0.f;
 #pragma unroll 2
-          for (int x = 0; x < m; ++x) {
-            const float w = s_weight[x][lane];
+            for (int x = 0; x < m; ++x) {
+              const float w = s_weight[x][lane];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = fmaf(s_buf[x * stride + (d + i) * 32 + lane], w, o[i]);
+              for (int i = 0; i < N; ++i) o[i] = fmaf(s_buf[x * stride + (d + i) * 32 + lane], w, o[i]);
+            }
+            if (base + m == n && r < nodes * G) {
+#pragma unroll
+              for (int i = 0; i < N; i += 8) {
+                const uint2 a = make_uint2(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv));
+                if constexpr (N == 4)
+                  *reinterpret_cast<uint2*>(dst + dim0 + d) = a;
+                else
+                  *reinterpret_cast<uint4*>(dst + dim0 + d + i) =
+                      make_uint4(a.x, a.y, pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+              }
+            }
           }
-          if (base + m == n && r < nodes * G)
-            *reinterpret_cast<uint2*>(dst + dim0 + d) = make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
-        }
+        };
+        if (dims == 16) join(std::integral_constant<int, 4>{});
+        else if (dims == 32) join(std::integral_constant<int, 8>{});
+        else join(std::integral_constant<int, 16>{});
       }
     }
   }

@@ -47,9 +47,9 @@ __device__ __forceinline__ uint32_t tree_keep32(const uint32_t* mask, int words,
 // within one that it began (place 2 * CTA + 1).  Every CTA writes its entries.
 constexpr int kTrMaxCtas = 160;               // (a B200 has 148 multiprocessors)
 struct TreePieces {
-  int head[kTrMaxCtas];                       // nodes of the unit that the share ends within, 0: none
-  int cont[kTrMaxCtas];                       // the share begins within a unit: 1, or 2 if it has the unit's last tile, too; 0: it does not
-  int2 unit[kTrMaxCtas];                      // where head is set: the unit's first row, its kv head
+  // x: nodes of the unit that the share ends within, 0: none; z, w: that unit's first row, its kv head.  y: the share begins within a
+  // unit: 1, or 2 if it has the unit's last tile, too; 0: it does not
+  int4 of[kTrMaxCtas];
 };
 
 // Partial results of one piece: 8 groups of 32 rows, each [128 dims][32 rows] and [max, sum][32 rows] in fp32, so that both kernels

@@ -262,9 +262,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
       ++n_pub;
     }
     if (!started) asm volatile("griddepcontrol.wait;" ::: "memory");
-    p.pieces->cont[blockIdx.x] = cont;
-    p.pieces->head[blockIdx.x] = head;
-    p.pieces->unit[blockIdx.x] = head_unit;
+    p.pieces->of[blockIdx.x] = make_int4(head, cont, head_unit.x, head_unit.y);
     if (ok) {
       const int is = n_pub % kSmItems;
       if (mbar_wait(&bar_item_empty[is], ((n_pub / kSmItems) & 1) ^ 1, abort_flag)) {
