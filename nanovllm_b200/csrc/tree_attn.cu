@@ -102,7 +102,7 @@ __device__ __forceinline__ void tree_cluster_store(uint32_t addr, float v) {
 }
 // What the CTAs of a cluster send one another, in the room of the rings: from each of them 128 / CTAs dims, then maxima and sums,
 // of 256 rows.
-constexpr int kTrClusterMax = 8;
+constexpr int kTrClusterLog = 3, kTrClusterMax = 1 << kTrClusterLog;
 static_assert(2 * (64 + 2) * 256 * 4 <= 7 * kTrTile && kTrClusterMax * (16 + 2) * 256 * 4 <= 7 * kTrTile, "inbox");
 
 template <bool kCluster>
@@ -153,11 +153,11 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   }
   __syncthreads();
   int c_nodes = 0, c_row = 0, c_head = 0, c_tiles = 0;       // kCluster: the cluster's unit
-  const int c_size = kCluster ? p.cluster : 1, c_rank = blockIdx.x % c_size;         // CTAs of a cluster: 2, 4 or 8
-  const int c_dims = 128 / c_size, c_inbox = (c_dims + 2) * 256;                        // floats of one sender
+  const int c_log = kCluster ? p.cluster_log : 0, c_size = 1 << c_log, c_rank = blockIdx.x & (c_size - 1);
+  const int c_dims = 128 >> c_log, c_inbox = (c_dims + 2) * 256;                        // floats of one sender
   if constexpr (kCluster) {
     // sequence i owns blocks of nodes [cu_q[i] / (2 * QT) + i, ...); there are few sequences
-    const int x = static_cast<int>(blockIdx.x / c_size), slot = x / p.Hkv;
+    const int x = static_cast<int>(blockIdx.x) >> c_log, slot = x / p.Hkv;
     c_head = x - slot * p.Hkv;
     int seq = 0;
 #pragma unroll 1
@@ -172,8 +172,8 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       s_bare = c_rank == 0 && c_tiles == 0;
       s_at[0][0] = s_at[1][0] = c_tiles > 0 ? seq : p.batch;
       s_at[0][1] = s_at[1][1] = block * p.Hkv + c_head;
-      s_at[0][2] = c_tiles * c_rank / c_size;
-      s_at[1][2] = c_tiles * (c_rank + 1) / c_size;
+      s_at[0][2] = c_tiles * c_rank >> c_log;
+      s_at[1][2] = c_tiles * (c_rank + 1) >> c_log;
     }
   } else
     tree_share<TcLine, kTrThreads>(p, 2 * QT, s_scan, s_at, &s_bare);
@@ -649,7 +649,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
 #pragma unroll
             for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), wb, __uint_as_float(a[i]) * wa));
             if constexpr (kCluster) {
-              const uint32_t to = tree_cluster_addr(inbox + (cch * 16 % c_dims) * 1024, cch * 16 / c_dims);
+              const uint32_t to = tree_cluster_addr(inbox + (cch * 16 & (c_dims - 1)) * 1024, cch * 16 >> (7 - c_log));
 #pragma unroll
               for (int i = 0; i < 16; ++i) tree_cluster_store(to + i * 1024, __uint_as_float(a[i]));
             } else if (part) {
@@ -686,25 +686,32 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     const int row = tid & 255, half = row >> 7, r = row & 127, t = r / G, node = half * QT + t;
     if (r < QT * G && node < c_nodes && c_tiles > 0) {
       // (with fewer tiles than CTAs some have sent nothing)
-      float M = -INFINITY;
-#pragma unroll 1
-      for (int x = 0; x < c_size; ++x)
-        if (c_tiles * (x + 1) / c_size > c_tiles * x / c_size) M = fmaxf(M, inbox[x * c_inbox + c_dims * 256 + row]);
+      float m[kTrClusterMax], l[kTrClusterMax], M = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kTrClusterMax; ++x) {
+        const bool sent = x < c_size && (c_tiles * (x + 1) >> c_log) > (c_tiles * x >> c_log);
+        m[x] = sent ? inbox[x * c_inbox + c_dims * 256 + row] : -INFINITY;
+        l[x] = sent ? inbox[x * c_inbox + (c_dims + 1) * 256 + row] : 0.f;
+        M = fmaxf(M, m[x]);
+      }
       const float ref = M == -INFINITY ? 0.f : M;
+      float sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kTrClusterMax; ++x) {
+        m[x] = fast_exp2(m[x] - ref);
+        sum = fmaf(l[x], m[x], sum);
+      }
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
       __nv_bfloat16* const dst = p.out + (static_cast<long long>(c_row + node) * p.H + c_head * G + (r - t * G)) * 128 + c_rank * c_dims;
 #pragma unroll 1
       for (int d = (tid >> 8) * 8; d < c_dims; d += 16) {
-        float sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int x = 0; x < c_size; ++x) {
-          if (c_tiles * (x + 1) / c_size == c_tiles * x / c_size) continue;
-          const float* const from = inbox + x * c_inbox + row;
-          const float w = fast_exp2(from[c_dims * 256] - ref);
-          sum = fmaf(from[(c_dims + 1) * 256], w, sum);
+        float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = fmaf(from[(d + i) * 256], w, o[i]);
+        for (int x = 0; x < kTrClusterMax; ++x) {
+          if (m[x] == 0.f) continue;             // (nothing sent, or nothing that counts)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = fmaf(inbox[x * c_inbox + (d + i) * 256 + row], m[x], o[i]);
         }
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
         uint4 v;
         v.x = pack_bf16(o[0] * inv, o[1] * inv);
         v.y = pack_bf16(o[2] * inv, o[3] * inv);
@@ -1023,10 +1030,10 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
     if (static_cast<long long>(bt_cols) * (block_size / kTrKv) > kTrClusterTiles[i] || units > tree_clusters_on_chip(i)) continue;
     rc = tree_configure<true>();
     if (rc) return rc;
-    p.cluster = kTrClusterMax >> i;
+    p.cluster_log = kTrClusterLog - i;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
-    tree_cluster_config(&cfg, attr, static_cast<unsigned>(units), static_cast<unsigned>(p.cluster), static_cast<cudaStream_t>(stream));
+    tree_cluster_config(&cfg, attr, static_cast<unsigned>(units), 1u << p.cluster_log, static_cast<cudaStream_t>(stream));
     const cudaError_t le = cudaLaunchKernelEx(&cfg, tree_attn_kernel<true>, p, map_q, map_k, map_v, map_k16, map_v16);
     g_launches.fetch_add(1);
     return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn(cluster) launch");

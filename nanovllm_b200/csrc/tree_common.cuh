@@ -20,7 +20,7 @@ struct TreeParams {
   int mask_words;                    // 32-bit words of a row
   int batch, total_q, H, Hkv, G;
   float scale_log2;
-  int cluster;                       // CTAs to a unit, where a cluster has one
+  int cluster_log;                   // where a cluster has a unit: log2 of its CTAs
   struct TreePieces* pieces;         // records of cut units
   float* partials;                   // [2 * CTAs] partial results
 };
