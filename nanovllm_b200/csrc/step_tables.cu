@@ -9,7 +9,10 @@
 // sequence i's j-th new block is free[n - 1 - (E_i + j)]: the list is a stack, and giving the same blocks back in the same order
 // leaves it as it was.  A few KB move, so the time is that of the dependent steps (lengths -> owned -> scan -> ids -> slots):
 // one cluster of 8 CTAs does all of them.  Each CTA scans the whole batch for itself and fills an eighth of the outputs; the
-// cluster's barrier stands between the last read of the old state and the first write of the new one.
+// cluster's barrier stands between the last read of the old state and the first write of the new one.  Us for 512 decodes, 40 prompts
+// and 96 trees, launches on end in a graph: 1 CTA 9.3, 24.6, 24.6; 2 CTAs 7.3, 16.2, 14.9; 4 6.3, 10.5, 9.9; 8 5.9, 7.5, 7.3, and started
+// early 5.6, 7.1, 6.6 (release 2.3).  Of the 4.9 on the device for the decodes 1.1 are the hash of the rows, 1.5 the two sums; of
+// the 5.9 for prompts 3.5 the tokens (four of a thread's tokens at a time: the same).
 #include <climits>
 
 #include "../../include/b200_attn.h"

@@ -23,6 +23,11 @@
 // which P replaced the scores, a half's next S had to wait for its P V: a chain of 3740 cycles a tile at 256 rows, of which the
 // softmax is 1990.
 // Every mbarrier wait is bounded.
+// Calls on end in a graph (with the join): 1 sequence of 1037 tokens, 9 nodes, 16/8 heads 10.6 us, in a cluster of 8 (of these 5 are the chain of
+// loads, one tile's S, softmax and P V, and 3.5 the two meetings and the join); 13 of 203 .. 3001, 5 .. 33 nodes, 32/8 31.9 us
+// (2.8 TB/s: 6 us until the first tiles are there, 7 the join); 4 of 24000 .. 40960, 33 .. 64 nodes, 8/2 45.8 us (2.9 TB/s, 560 TFLOP/s);
+// 128 of 512 .. 4096, 64 nodes, 32/8 324 us (4.1 TB/s, 950 TFLOP/s; 340 where the power cap sets in, up to 400 with L2 flushed between
+// calls): the softmax chain of a tile, about 3100 cycles for both halves against 2048 of tensor work.
 #include <atomic>
 
 #include "../../include/b200_attn.h"
@@ -162,7 +167,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     int seq = 0;
 #pragma unroll 1
     for (int i = 1; i < p.batch; ++i)
-      if (max(0, min(__ldg(p.cu_q + i), p.total_q)) / (2 * QT) + i <= slot) seq = i;
+      if (max(0, min(p.cu_q[i], p.total_q)) / (2 * QT) + i <= slot) seq = i;
     const TreeSeq s = tree_seq<TcLine>(p, 2 * QT, seq);
     const int block = slot - (s.q_begin / (2 * QT) + seq), node0 = block * 2 * QT;
     c_nodes = block >= 0 ? min(s.nodes - node0, 2 * QT) : 0;
@@ -732,8 +737,9 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
 }
 
 // Units that a cut ran through.  A task is (unit, group of 32 rows, some of the dims: the fewer units, the fewer); its partial results
-// come as bulk copies, all under way at once.  What takes time here is round trips to L2 and fetching the code, which is new
-// for every launch: so every warp reads all records (five words a lane) and finds its unit and pieces by bits of ballots.
+// come as bulk copies, all under way at once.  What takes time here is round trips to L2 (records 0.4 us, pieces 1.4, of 6.6 at 4 long
+// contexts, of 4 at 13 trees) and fetching the code, which is new for every launch (going through it once ahead of the wait: the same):
+// so every warp reads all records (five a lane) and finds its unit and pieces by bits of ballots.
 constexpr int kTrJoinThreads = 128;
 constexpr int kTrJoinCtas = 5;                // per SM
 constexpr int kTrJoinPieces = 16;             // of 16 dims; 2 of 128
@@ -884,11 +890,12 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
 
 constexpr size_t kTrSmem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTile;
 // Sizes of clusters, and how wide (in key tiles) the table may be for each: what the host knows of the lengths.  Us with the join |
-// with clusters, calls on end:
-//   8   1 sequence of 300, 4000, 12000 tokens, 9 nodes, 16/8 heads   14.0, 18.3, 23.1 | 9.6, 12.2, 18.8; 60 nodes, 8/2 heads
-//       16.3, 22.4, 32.4 | 13.2, 20.3, 31.6, and of 16000 32.5 | 37.5
-//   4   4 of 500, 2000, 4000, 20 nodes, 32/8   18.6, 21.9, 28.1 | 11.2, 16.5, 24.8; of 200 .. 4000, 300 .. 8000   21.4, 28.1 | 22.7, 36.3
-//   2   9 of 500, 2000, 4000, 9 nodes, 16/8    17.2, 26.4, 38.2 | 14.0, 22.0, 32.8; 6 of 200 .. 4000, 300 .. 8000   24.1, 32.1 | 23.4, 37.2
+// with clusters, calls on end in a graph:
+//   8   1 sequence of 300, 4000, 12000 tokens, 9 nodes, 16/8 heads   13.0, 16.9, 21.5 | 9.5, 12.2, 19.0; 60 nodes, 8/2 heads
+//       15.4, 20.5, 29.9 | 13.2, 20.4, 31.5, and of 16000 30.0 | 37.5
+//   4   4 of 500, 2000, 4000, 20 nodes, 32/8   16.6, 20.1, 26.2 | 10.4, 15.6, 23.8; of 200 .. 4000   19.4 | 21.8
+//   2   9 of 500, 2000, 4000, 9 nodes, 16/8    15.8, 24.7, 36.4 | 12.8, 21.4, 31.7; 6 of 200 .. 4000   21.0 | 22.4
+// (What clusters lose, they lose where lengths differ; wider tables make that worse: 4 of 300 .. 8000 lost 8 us, 6 of them 5.)
 constexpr int kTrClusterSizes = 3;
 constexpr int kTrClusterTiles[kTrClusterSizes] = {128, 40, 32};
 
@@ -1039,9 +1046,10 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
     return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn(cluster) launch");
   }
   // Few nodes to a sequence: tree_small.cu, up to 12 rows on average.  Us of this kernel | that one, calls on end: 256 sequences of
-  // 100 .. 2048 tokens at 16/8 heads, 1 node 210 | 180, 4 nodes 214 | 189, 8 nodes (16 rows) 224 | 215, 12 nodes 231 | 395; 128 of
-  // 500 .. 4096 at 32/8, 4 nodes (16 rows) 219 | 211; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 78 | 74; but, with 16 rows, 20 of
-  // 300 .. 2000 at 32/8, 4 nodes 31.8 | 34.3, and 64 of 500 .. 3000 at 4/2, 2 .. 14 nodes 34.1 | 38.5.
+  // 100 .. 2048 tokens at 16/8 heads, 1 node 211 | 179, 4 nodes 216 | 189, 6 nodes (12 rows) 219 | 196, 8 nodes (16 rows) 224 | 215, 12 nodes
+  // 231 | 395; 128 of 500 .. 4096 at 32/8, 1 node 205 | 190; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 85 | 73; 64 of
+  // 500 .. 3000 at 4/2, 2 .. 10 nodes (12 rows) 31.9 | 32.9; but, with 16 rows, 20 of 300 .. 2000 at 32/8, 4 nodes 31.8 | 34.3, and 64 of
+  // 500 .. 3000 at 4/2, 2 .. 14 nodes 34.1 | 38.5.
   if (G <= 16 && static_cast<long long>(total_q) * G <= 12LL * batch) {
     rc = make_tokens_heads_map(&map_k, k_cache, rows, num_kv_heads, row, 64);
     if (!rc) rc = make_tokens_heads_map(&map_v, v_cache, rows, num_kv_heads, row, 64);

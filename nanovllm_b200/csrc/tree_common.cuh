@@ -65,9 +65,9 @@ struct TreeSeq {
 template <typename L>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int block_nodes, int i) {
   TreeSeq s;
-  s.q_begin = max(0, min(__ldg(p.cu_q + i), p.total_q));
-  s.nodes = max(0, min(__ldg(p.cu_q + i + 1), p.total_q) - s.q_begin);
-  s.Lk = max(0, min(__ldg(p.context_lens + i), p.bt_cols * p.block_size));
+  s.q_begin = max(0, min(p.cu_q[i], p.total_q));
+  s.nodes = max(0, min(p.cu_q[i + 1], p.total_q) - s.q_begin);
+  s.Lk = max(0, min(p.context_lens[i], p.bt_cols * p.block_size));
   s.tiles = (s.Lk + L::kKeys - 1) / L::kKeys;
   s.blocks = s.tiles > 0 ? (s.nodes + block_nodes - 1) / block_nodes : 0;
   s.last_split = s.nodes - (s.blocks - 1) * block_nodes <= block_nodes / 2;
@@ -107,7 +107,7 @@ struct TreeRows {
   }
   __device__ __forceinline__ int next(const TreeParams& p) {
     if (in_block <= 0) {
-      const int blk = __ldg(blocks++);
+      const int blk = *blocks++;
       row = blk >= 0 && blk < p.num_blocks ? blk * p.block_size - in_block : -(1 << 30);
       in_block += p.block_size;
     }

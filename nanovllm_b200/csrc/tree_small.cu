@@ -9,6 +9,8 @@
 // groups take the tiles in turn, 16 keys of a tile to a warp: a byte of shared memory is read by one warp only.  At the end of
 // a unit a group leaves its accumulators in the stage of its last tile, which goes back to the ring when the epilogue warps have
 // joined them: the consumers go on with the next unit meanwhile, and the room costs nothing.
+//
+// 256 chains of 4 nodes on 100 .. 2048 tokens at 16/8 heads: 182 to 189 us with the join, 6.0 to 6.2 TB/s (a copy: 6.55); 1 node 179.
 #include <atomic>
 
 #include "../../include/b200_attn.h"

@@ -15,6 +15,7 @@ from nanovllm_b200 import _lib
 from nanovllm_b200.engine.block_tables import DeviceBlockTables, StepTables
 from nanovllm_b200.engine.tree_decode import accept_tree, compact_kvcache
 from oracle.tree_oracle import BlockState, accept_tree_ref, compact_ref, tree_attn_ref
+from test_early_start import _compare, late_copy  # noqa: F401  (late_copy is a fixture)
 
 DEV = "cuda:0"
 BOUND = 2.0 ** -8 + 2.0 ** -11
@@ -610,3 +611,75 @@ def test_two_graphs_on_two_streams():
     for c, (_, out) in zip(cases, held):
         check_attention(c, out)
     status_ok()
+
+
+# ---- early starts ----------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,hkv,ctx,nodes", [(16, 8, [1037], [9]), (32, 8, [700, 300, 500, 900, 40], [20, 33, 5, 64, 12]),
+                                             (8, 1, [200 + 7 * i for i in range(130)], [1] * 130), (8, 4, [150 + i for i in range(60)], [12] * 60)])
+def test_attention_behind_a_kernel_that_writes_its_rows(late_copy, H, hkv, ctx, nodes):
+    """Rows, masks and the cache come from a kernel that lets this one start before it writes them (clusters, cut units and the
+    join, few nodes)."""
+    c = attention_case(H, hkv, ctx, nodes, 71, poison=False)
+    late = dict(q=c["q"].contiguous(), k=c["k"], v=c["v"], masks=c["masks"])
+    late = {n: t.to(DEV) for n, t in late.items()}
+    cu, lens, tables = i32(c["cu"]), i32(ctx), i32(c["tables"])
+    _compare(late_copy, {n: torch.zeros_like(t) for n, t in late.items()}, late, lambda: None,
+             lambda m, _: (nanovllm_b200.tree_attention(m["q"], m["k"], m["v"], cu, lens, tables, m["masks"], c["scale"], hkv),))
+    status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,seed", [(1, 1), (40, 2), (700, 3)])
+def test_tables_walk_and_moves_behind_a_kernel_that_writes_their_inputs(late_copy, batch, seed):
+    rng = random.Random(seed)
+    sizes = [rng.randrange(1, 20) for _ in range(batch)]
+    total, cols = sum(sizes), 4
+    rows = rng.sample(range(batch + 5), batch)
+    cached = [rng.randrange(700) for _ in sizes]
+    parents = random_parents(sizes, rng)
+    cu = [0]
+    for s in sizes:
+        cu.append(cu[-1] + s)
+    zeros = lambda late: {n: torch.zeros_like(t) for n, t in late.items()}  # noqa: E731
+    fresh = lambda: DeviceBlockTables.create(batch + 5, cols, cols * batch + 3, 256, DEV)  # noqa: E731
+    late = dict(rows=i32(rows), cached=i32(cached), new=i32(sizes), parents=i32(parents))
+
+    def step(m, s):
+        return (*s.step(m["rows"], m["cached"], m["new"], total, m["parents"], 1), s.tables, s.owned, s.free_blocks, s.pool)
+    _compare(late_copy, zeros(late), late, fresh, step)
+
+    def taken():
+        s = fresh()
+        s.step(late["rows"], late["cached"], late["new"], total)
+        return s
+
+    def release(m, s):
+        s.release(m["rows"], m["keep"])
+        return s.tables, s.owned, s.free_blocks, s.pool
+    keep = dict(rows=late["rows"], keep=i32([rng.randrange(900) for _ in sizes]))
+    _compare(late_copy, zeros(keep), keep, taken, release)
+    walk = dict(draft=i64([rng.randrange(3) for _ in parents]), target=i64([rng.randrange(3) for _ in parents]), parents=late["parents"], cu=i32(cu),
+                cached=late["cached"], context=i32([a + b for a, b in zip(cached, sizes)]))
+    _compare(late_copy, zeros(walk), walk, lambda: None,
+             lambda m, _: tuple(accept_tree(m["draft"], m["target"], m["parents"], m["cu"], m["cached"], m["context"], 6)))
+    paths = [sorted(rng.sample(range(20), 6)) for _ in sizes]
+    blocks = cols * batch
+    cache = torch.randint(-30000, 30000, (blocks, 256, 1, 8), dtype=torch.int16, device=DEV)
+    moves = dict(path=i32(paths), accepted=i32([rng.randrange(7) for _ in sizes]), start=late["cached"], tables=torch.arange(blocks, dtype=torch.int32, device=DEV).view(batch, cols))
+
+    def compact(m, mine):
+        compact_kvcache(mine, m["path"], m["accepted"], m["start"], m["tables"])
+        return (mine,)
+    _compare(late_copy, zeros(moves), moves, cache.clone, compact)
+    status_ok()
+
+
+@pytest.mark.gpu
+def test_compaction_from_no_place():
+    """Negative start lengths (the largest, too) move nothing."""
+    cache = torch.arange(2 * 256 * 8, dtype=torch.int32, device=DEV).view(2, 256, 1, 8)
+    want = cache.clone()
+    compact_kvcache(cache, i32([[0, 3, 2 ** 31 - 1]] * 3), i32([3, 3, 3]), i32([-1, -2 ** 31, -3]), i32([[0], [1], [0]]))
+    torch.cuda.synchronize()
+    assert torch.equal(cache, want)
