@@ -833,10 +833,8 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
           tree_bulk_load(s_buf + tid * stride, from + dim0 * 32, dims * 128, &s_bar);
           tree_bulk_load(s_buf + tid * stride + dims * 32, from + 128 * 32, 256, &s_bar);
         }
-        if (!mbar_wait(&s_bar, loads & 1, &s_abort)) {
-          if (tid == 0) atomicExch(&g_status_tree, 1);
-          return;
-        }
+        // (a wait that gave up leaves the barriers below complete: nobody leaves)
+        if (!mbar_wait(&s_bar, loads & 1, &s_abort)) atomicExch(&g_status_tree, 1);
         ++loads;
         // every warp for itself: the new maximum and sum; the weights are shared out
         float top = M;

@@ -140,7 +140,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
   unsigned char* const sQ = smem + kSmStages * kSmStage;            // [2][4 KiB]
   __shared__ __align__(8) uint64_t bar_full[kSmStages], bar_empty[kSmStages];
   __shared__ __align__(8) uint64_t bar_item_full[kSmItems], bar_item_empty[kSmItems], bar_q_full[2], bar_q_empty[2];
-  __shared__ __align__(8) uint64_t bar_state_full[2], bar_state_free[2];
+  __shared__ __align__(8) uint64_t bar_state_full[2], bar_state_free[2], bar_read[2];
   __shared__ float s_ml[8][16][2];                                  // consumer warps' maxima (log2 units) and sums
   __shared__ __align__(16) SmallItem s_item[kSmItems];
   __shared__ unsigned s_scan[kSmThreads / 32];
@@ -159,6 +159,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
       mbar_init(&bar_q_empty[i], 8);
       mbar_init(&bar_state_full[i], 4);
       mbar_init(&bar_state_free[i], 3);
+      mbar_init(&bar_read[i], 4);
     }
     mbar_fence_init();
     s_at[0][0] = s_at[1][0] = p.batch;
@@ -336,6 +337,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
         if (j + 2 < it.n) {
           if (lane == 0) mbar_arrive(&bar_empty[stage]);
         } else {
+          if (lane == 0) mbar_arrive(&bar_read[group]);
           last = stage;
         }
       }
@@ -348,7 +350,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
       a.l1 += __shfl_xor_sync(0xffffffffu, a.l1, 1);
       a.l1 += __shfl_xor_sync(0xffffffffu, a.l1, 2);
       if (!mbar_wait(&bar_state_free[group], (n_state & 1) ^ 1, abort_flag)) break;
-      named_bar_sync(1 + group, 128);
+      if (!mbar_wait(&bar_read[group], n_state & 1, abort_flag)) break;
       // ([16 rows][128 dims], groups of 8 dims in another order in each row, so that a store meets no bank twice)
       float* const state = reinterpret_cast<float*>(stages + last * kSmStage + slab * kSmSub);
 #pragma unroll
@@ -367,6 +369,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
       if (lane == 0) mbar_arrive(&bar_state_full[group]);
       ++n_state;
     }
+    if (*abort_flag) atomicExch(&g_status_tree_small, 1);
     return;
   }
 
@@ -465,6 +468,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
       }
     }
   }
+  if (*abort_flag) atomicExch(&g_status_tree_small, 1);
 }
 
 int launch_tree_small(const TreeParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_k16, const CUtensorMap& map_v16,
