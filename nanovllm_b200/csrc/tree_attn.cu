@@ -177,8 +177,9 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       s_bare = c_rank == 0 && c_tiles == 0;
       s_at[0][0] = s_at[1][0] = c_tiles > 0 ? seq : p.batch;
       s_at[0][1] = s_at[1][1] = block * p.Hkv + c_head;
-      s_at[0][2] = c_tiles * c_rank >> c_log;
-      s_at[1][2] = c_tiles * (c_rank + 1) >> c_log;
+      // (what is left over goes to the CTAs in front: the last has the tile with the masks)
+      s_at[0][2] = (c_tiles * c_rank + c_size - 1) >> c_log;
+      s_at[1][2] = (c_tiles * (c_rank + 1) + c_size - 1) >> c_log;
     }
   } else
     tree_share<TcLine, kTrThreads>(p, 2 * QT, s_scan, s_at, &s_bare);
@@ -694,7 +695,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       float m[kTrClusterMax], l[kTrClusterMax], M = -INFINITY;
 #pragma unroll
       for (int x = 0; x < kTrClusterMax; ++x) {
-        const bool sent = x < c_size && (c_tiles * (x + 1) >> c_log) > (c_tiles * x >> c_log);
+        const bool sent = x < c_size && (c_tiles * (x + 1) + c_size - 1) >> c_log > (c_tiles * x + c_size - 1) >> c_log;
         m[x] = sent ? inbox[x * c_inbox + c_dims * 256 + row] : -INFINITY;
         l[x] = sent ? inbox[x * c_inbox + (c_dims + 1) * 256 + row] : 0.f;
         M = fmaxf(M, m[x]);
