@@ -105,8 +105,11 @@ __device__ __forceinline__ uint32_t tree_cluster_addr(uint32_t addr, uint32_t ra
 __device__ __forceinline__ void tree_cluster_store(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
-// What the CTAs of a cluster send one another, in the room of the rings: from each of them 128 / CTAs dims, then maxima and sums,
-// of 256 rows.
+__device__ __forceinline__ void tree_cluster_store4(uint32_t addr, const uint32_t* v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// What the CTAs of a cluster send one another, in the room of the rings: from each of them 128 / CTAs dims (4 of a row side by
+// side, so that a store or load of a warp moves 512 bytes), then maxima and sums, of 256 rows.
 constexpr int kTrClusterLog = 3, kTrClusterMax = 1 << kTrClusterLog;
 static_assert(2 * (64 + 2) * 256 * 4 <= 7 * kTrTile && kTrClusterMax * (16 + 2) * 256 * 4 <= 7 * kTrTile, "inbox");
 
@@ -624,12 +627,12 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
           const int t = r / G;
           __nv_bfloat16* const dst = p.out + (static_cast<long long>(it.q_row + turn * QT + t) * p.H + it.h * G + (r - t * G)) * 128;
           float* const part = kCluster || it.partial < 0 ? nullptr : p.partials + static_cast<long long>(it.partial) * kTrPartial + (turn * 4 + quarter) * kTrGroup + lane;
-          const uint32_t inbox = smem_u32(smem) + (c_rank * c_inbox + turn * 128 + r) * 4;
+          const uint32_t inbox = smem_u32(smem) + c_rank * c_inbox * 4, in_row = turn * 128 + r;
           if constexpr (kCluster) {
 #pragma unroll 1
             for (int x = 0; x < c_size; ++x) {
-              tree_cluster_store(tree_cluster_addr(inbox + c_dims * 1024, x), M);
-              tree_cluster_store(tree_cluster_addr(inbox + (c_dims + 1) * 1024, x), sum);
+              tree_cluster_store(tree_cluster_addr(inbox + c_dims * 1024 + in_row * 4, x), M);
+              tree_cluster_store(tree_cluster_addr(inbox + (c_dims + 1) * 1024 + in_row * 4, x), sum);
             }
           } else if (part) {
             part[128 * 32] = M;
@@ -655,9 +658,9 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
 #pragma unroll
             for (int i = 0; i < 16; ++i) a[i] = __float_as_uint(fmaf(__uint_as_float(b[i]), wb, __uint_as_float(a[i]) * wa));
             if constexpr (kCluster) {
-              const uint32_t to = tree_cluster_addr(inbox + (cch * 16 & (c_dims - 1)) * 1024, cch * 16 >> (7 - c_log));
+              const uint32_t to = tree_cluster_addr(inbox + (cch * 16 & (c_dims - 1)) * 1024 + in_row * 16, cch * 16 >> (7 - c_log));
 #pragma unroll
-              for (int i = 0; i < 16; ++i) tree_cluster_store(to + i * 1024, __uint_as_float(a[i]));
+              for (int i = 0; i < 16; i += 4) tree_cluster_store4(to + i * 1024, a + i);
             } else if (part) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) part[(cch * 16 + i) * 32] = __uint_as_float(a[i]);
@@ -716,7 +719,13 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         for (int x = 0; x < kTrClusterMax; ++x) {
           if (m[x] == 0.f) continue;             // (nothing sent, or nothing that counts)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = fmaf(inbox[x * c_inbox + (d + i) * 256 + row], m[x], o[i]);
+          for (int i = 0; i < 8; i += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(inbox + x * c_inbox + (d + i) * 256 + row * 4);
+            o[i] = fmaf(v.x, m[x], o[i]);
+            o[i + 1] = fmaf(v.y, m[x], o[i + 1]);
+            o[i + 2] = fmaf(v.z, m[x], o[i + 2]);
+            o[i + 3] = fmaf(v.w, m[x], o[i + 3]);
+          }
         }
         uint4 v;
         v.x = pack_bf16(o[0] * inv, o[1] * inv);
