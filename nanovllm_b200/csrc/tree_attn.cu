@@ -23,8 +23,8 @@
 // which P replaced the scores, a half's next S had to wait for its P V: a chain of 3740 cycles a tile at 256 rows, of which the
 // softmax is 1990.
 // Every mbarrier wait is bounded.
-// Calls on end in a graph (with the join): 1 sequence of 1037 tokens, 9 nodes, 16/8 heads 10.6 us, in a cluster of 8 (of these 5 are the chain of
-// loads, one tile's S, softmax and P V, and 3.5 the two meetings and the join); 13 of 203 .. 3001, 5 .. 33 nodes, 32/8 31.9 us
+// Calls on end in a graph (with the join): 1 sequence of 1037 tokens, 9 nodes, 16/8 heads 9.7 us, in a cluster of 8 (of these 5 are the chain of
+// loads, a tile's S, softmax and P V, and 3 the two meetings and the join); 13 of 203 .. 3001, 5 .. 33 nodes, 32/8 31.9 us
 // (2.8 TB/s: 6 us until the first tiles are there, 7 the join); 4 of 24000 .. 40960, 33 .. 64 nodes, 8/2 45.8 us (2.9 TB/s, 560 TFLOP/s);
 // 128 of 512 .. 4096, 64 nodes, 32/8 324 us (4.1 TB/s, 950 TFLOP/s; 340 where the power cap sets in, up to 400 with L2 flushed between
 // calls): the softmax chain of a tile, about 3100 cycles for both halves against 2048 of tensor work.
@@ -899,10 +899,10 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
 constexpr size_t kTrSmem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTile;
 // Sizes of clusters, and how wide (in key tiles) the table may be for each: what the host knows of the lengths.  Us with the join |
 // with clusters, calls on end in a graph:
-//   8   1 sequence of 300, 4000, 12000 tokens, 9 nodes, 16/8 heads   13.0, 16.9, 21.5 | 9.5, 12.2, 19.0; 60 nodes, 8/2 heads
-//       15.4, 20.5, 29.9 | 13.2, 20.4, 31.5, and of 16000 30.0 | 37.5
-//   4   4 of 500, 2000, 4000, 20 nodes, 32/8   16.6, 20.1, 26.2 | 10.4, 15.6, 23.8; of 200 .. 4000   19.4 | 21.8
-//   2   9 of 500, 2000, 4000, 9 nodes, 16/8    15.8, 24.7, 36.4 | 12.8, 21.4, 31.7; 6 of 200 .. 4000   21.0 | 22.4
+//   8   1 sequence of 300, 4000, 12000 tokens, 9 nodes, 16/8 heads   13.0, 16.9, 21.5 | 9.5, 12.0, 18.4; 60 nodes, 8/2 heads
+//       15.4, 20.5, 29.9 | 13.1, 20.3, 29.8, and of 16000 30.0 | 37.5
+//   4   4 of 500, 2000, 4000, 20 nodes, 32/8   16.6, 20.1, 26.2 | 10.1, 15.6, 23.4; of 200 .. 4000   19.4 | 21.8
+//   2   9 of 500, 2000, 4000, 9 nodes, 16/8    15.8, 24.7, 36.4 | 12.8, 20.8, 31.7; 6 of 200 .. 4000   21.0 | 22.4
 // (What clusters lose, they lose where lengths differ; wider tables make that worse: 4 of 300 .. 8000 lost 8 us, 6 of them 5.)
 constexpr int kTrClusterSizes = 3;
 constexpr int kTrClusterTiles[kTrClusterSizes] = {128, 40, 32};
