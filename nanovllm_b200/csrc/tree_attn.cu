@@ -29,6 +29,8 @@
 // 128 of 512 .. 4096, 64 nodes, 32/8 324 us (4.1 TB/s, 950 TFLOP/s; 340 where the power cap sets in, up to 400 with L2 flushed between
 // calls): the softmax chain of a tile, about 3100 cycles for both halves against 2048 of tensor work.
 #include <atomic>
+#include <cmath>
+#include <limits>
 
 #include "../../include/b200_attn.h"
 #include "tc_wait.cuh"
@@ -415,7 +417,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
     const int r = quarter * 32 + lane;                  // row of the tile
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tmem_s = tmem + lane_base, tmem_p = tmem + 128 + hx * 64 + lane_base, tmem_o = tmem + 256 + hx * 128 + lane_base;
-    const float c = p.scale_log2;
+    const float c = p.scale_abs;
     int n_item = 0, ns = 0, n_fin = 0;
     int v_at = 0, v_ph = 0;                             // place and phase in the V ring of the unit's last tile
     int v_next = 0;                                     // (tiles so far, modulo the ring's two turns)
@@ -449,19 +451,19 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         const int key0 = (it.t0 + (it.split ? 2 * j + mine : j)) * kTrKv;
         if (active) {
           tc::fence_after_sync();
-          if (key0 + kTrKv > min(it.first, it.Lk)) {
-            // the tile reaches the nodes: masked scores go back over S first (rolled: the hot code stays short)
+          if (key0 + kTrKv > min(it.first, it.Lk) || p.flip) {
+            // the tile reaches the nodes, or the scale is negative: masked or turned scores go back over S first (rolled: the hot
+            // code stays short)
 #pragma unroll 1
             for (int cch = 0; cch < 4; ++cch) {
               const int col = key0 + cch * 32;
               const uint32_t keep = chain || row_ok ? tree_keep32(mask, p.mask_words, node, col - it.first, it.Lk - col) : 0u;
-              if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
+              if (__all_sync(0xffffffffu, keep == 0xffffffffu) && !p.flip) continue;
               uint32_t v[32];
               tc::ld_32x32b_x32(tmem_s + cch * 32, v);
               tc::wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!((keep >> i) & 1)) v[i] = 0xff800000u;   // -inf
+              for (int i = 0; i < 32; ++i) v[i] = (keep >> i) & 1 ? v[i] ^ p.flip : 0xff800000u;   // (-inf)
               tc::st_32x32b_x32(tmem_s + cch * 32, v);
             }
             tc::wait_st();
@@ -1023,6 +1025,8 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.Hkv = num_kv_heads;
   p.G = G;
   p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_abs = scale == 0.f ? std::numeric_limits<float>::denorm_min() : std::fabs(p.scale_log2);
+  p.flip = scale < 0.f ? 0x80000000u : 0u;
   // the longest that the line of key tiles can be (table widths are all that the host knows of the lengths)
   const double blocks = total_q / (G <= 16 ? 16 / G : 2 * (128 / G)) + batch;
   const double line = num_kv_heads * blocks * (static_cast<double>(bt_cols) * (block_size / 64) * TcLine::kTilePair + TcLine::kUnitPair);

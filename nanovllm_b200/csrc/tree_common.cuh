@@ -20,6 +20,10 @@ struct TreeParams {
   int mask_words;                    // 32-bit words of a row
   int batch, total_q, H, Hkv, G;
   float scale_log2;
+  // The tcgen05 kernel takes the maximum of unscaled scores, which wants a positive scale: it is scale_abs (of 0 the least number
+  // above, so that -inf stays -inf), and `flip`, the sign bit of a negative one, goes over the scores.
+  float scale_abs;
+  uint32_t flip;
   int cluster_log;                   // where a cluster has a unit: log2 of its CTAs
   struct TreePieces* pieces;         // records of cut units
   float* partials;                   // [2 * CTAs] partial results
