@@ -145,9 +145,9 @@ int b200_decode_attn_static(const void* q, int64_t q_row_stride, const void* k_c
  * Sequences with Lq_i == 0 produce no rows.  out is (total_q, num_heads, 128) contiguous bf16.
  * max_seqlen_q / max_seqlen_k are the host-side bounds the caller already has
  * (nanovllm/utils/context.py:9-10).  kernel_variant: 0 = default (the persistent tcgen05 kernel
- * when 128 % (num_heads / num_kv_heads) == 0 and the batch is not so short that the mma.sync kernel is through it sooner,
- * else the mma.sync kernel), 1 = force the mma.sync
- * kernel, 2 = force the tcgen05 kernel (B200_ERR_BAD_SHAPE if it cannot take the shape).  Launches
+ * when 128 % (num_heads / num_kv_heads) == 0, the scale is positive and the batch is not so short that the mma.sync kernel is
+ * through it sooner, else the mma.sync kernel), 1 = force the mma.sync
+ * kernel, 2 = force the tcgen05 kernel (B200_ERR_BAD_SHAPE if it cannot take the shape or the scale).  Launches
  * of the tcgen05 kernel share one device-side ticket counter: do not overlap two of them on one
  * GPU.  The persistent kernel
  * writes `out` through TMA stores: out must be 16-byte aligned (as every tensor here). */

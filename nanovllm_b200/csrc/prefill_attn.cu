@@ -71,9 +71,10 @@ static int prefill(const void* q, int64_t q_row_stride, const void* k, const voi
 
   if (kernel_variant < 0 || kernel_variant > 2)
     return set_error(kErrBadShape, "prefill_attn: kernel_variant must be 0 .. 2");
-  const bool tc_ok = 128 % G == 0;
+  // (the tcgen05 kernel takes a row's maximum in front of the scale, so it needs a positive one; the other takes any)
+  const bool tc_ok = 128 % G == 0 && scale > 0.f;
   if (kernel_variant == 2 && !tc_ok)
-    return set_error(kErrBadShape, "prefill_attn: the tcgen05 kernel needs 128 %% (num_heads / num_kv_heads) == 0 (got %d)", G);
+    return set_error(kErrBadShape, "prefill_attn: the tcgen05 kernel needs 128 %% (num_heads / num_kv_heads) == 0 (got %d) and a positive scale", G);
   const PrefillChoice choice = prefill_choice(total_q, batch, num_kv_heads, G, max_seqlen_k);
   const bool use_tc = kernel_variant == 2 || (kernel_variant == 0 && tc_ok && choice.tc);
   const uint32_t kv_box = use_tc ? 128 : 64;
