@@ -307,7 +307,8 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         if (t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) {
           s_item[is].seq = -1;
           mbar_arrive(&bar_item_full[is]);
-          // every role has taken it (kCluster: the output warps do so behind the meeting that this warp is to come to)
+          // Every role has taken it, so all their waits have ended.  (kCluster: the output warps would take it behind the meeting that
+          // this warp is to come to, so they say so in front of it, where their last wait is behind them.)
           if (!kCluster) t2_wait_timed(&bar_item_empty[is], (n_pub / kTrItems) & 1, abort_flag);
         }
       }
@@ -451,19 +452,32 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         const int key0 = (it.t0 + (it.split ? 2 * j + mine : j)) * kTrKv;
         if (active) {
           tc::fence_after_sync();
-          if (key0 + kTrKv > min(it.first, it.Lk) || p.flip) {
-            // the tile reaches the nodes, or the scale is negative: masked or turned scores go back over S first (rolled: the hot
-            // code stays short)
+          if (p.flip) {
+            // a negative scale: scores of the other sign over S (a pass of its own: in the one below it cost all calls 0.5 us)
+#pragma unroll 1
+            for (int cch = 0; cch < 8; ++cch) {
+              uint32_t v[16];
+              tc::ld_32x32b_x16(tmem_s + cch * 16, v);
+              tc::wait_ld();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] ^= p.flip;
+              tc::st_32x32b_x16(tmem_s + cch * 16, v);
+            }
+            tc::wait_st();
+          }
+          if (key0 + kTrKv > min(it.first, it.Lk)) {
+            // the tile reaches the nodes: masked scores go back over S first (rolled: the hot code stays short)
 #pragma unroll 1
             for (int cch = 0; cch < 4; ++cch) {
               const int col = key0 + cch * 32;
               const uint32_t keep = chain || row_ok ? tree_keep32(mask, p.mask_words, node, col - it.first, it.Lk - col) : 0u;
-              if (__all_sync(0xffffffffu, keep == 0xffffffffu) && !p.flip) continue;
+              if (__all_sync(0xffffffffu, keep == 0xffffffffu)) continue;
               uint32_t v[32];
               tc::ld_32x32b_x32(tmem_s + cch * 32, v);
               tc::wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = (keep >> i) & 1 ? v[i] ^ p.flip : 0xff800000u;   // (-inf)
+              for (int i = 0; i < 32; ++i)
+                if (!((keep >> i) & 1)) v[i] = 0xff800000u;   // -inf
               tc::st_32x32b_x32(tmem_s + cch * 32, v);
             }
             tc::wait_st();
