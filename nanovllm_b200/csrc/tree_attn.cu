@@ -231,6 +231,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       TreeRows<TcLine> rows = {};
       const int end_seq = s_at[1][0], end_unit = s_at[1][1], end_tile = s_at[1][2];
       int n_pub = 0, q_use = 0, turn = 0, k_at = 0, k_ph = 1;
+      int halves = 0;                 // kCluster: halves with work
       bool ok = true, started = false;
 #pragma unroll 1
       while (ok && seq < p.batch) {
@@ -267,6 +268,7 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         mbar_arrive(&bar_item_full[is]);
         ++n_pub;
         if (split) turn ^= (t1 - t0) & 1;
+        if constexpr (kCluster) halves = split && t1 - t0 == 1 ? 1 : 2;     // (a CTA has one item)
         rows.start(p, owner, t0);
         int row = rows.next(p), left = s.Lk - t0 * kTrKv;
         if (!started) {
@@ -307,9 +309,12 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         if (t2_wait_timed(&bar_item_empty[is], ((n_pub / kTrItems) & 1) ^ 1, abort_flag)) {
           s_item[is].seq = -1;
           mbar_arrive(&bar_item_full[is]);
-          // Every role has taken it, so all their waits have ended.  (kCluster: the output warps would take it behind the meeting that
-          // this warp is to come to, so they say so in front of it, where their last wait is behind them.)
-          if (!kCluster) t2_wait_timed(&bar_item_empty[is], (n_pub / kTrItems) & 1, abort_flag);
+          // Every role has taken it, so all their waits have ended.  (kCluster: the output warps take it behind the meeting that this
+          // warp is to come to; in front of it their last wait is for the accumulators.)
+          if constexpr (kCluster) {
+            for (int i = 0; i < halves; ++i) t2_wait_timed(&bar_o_final[i], 0, abort_flag);
+          } else
+            t2_wait_timed(&bar_item_empty[is], (n_pub / kTrItems) & 1, abort_flag);
         }
       }
     } else if (warp == 1 && lane == 0) {
