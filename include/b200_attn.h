@@ -257,7 +257,9 @@ int64_t b200_tree_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32
  * that the sequence does not have mean nothing; nodes from 64 * mask_words on are seen by none.  A row that sees nothing
  * (context_lens[i] <= 0 among them) gives zeros.  GQA, scale and numerics as b200_decode_attn; out (total_q, num_heads, 128)
  * contiguous; rows outside cu_seqlens_q are left as they are.  Keys and values of a sequence's positions must be finite, seen or
- * not.  At most 128 query heads per kv head, mask_words at most 4.  The same inputs give the same bits on every call. */
+ * not.  At most 128 query heads per kv head, mask_words at most 4.  Where the call does not fit into thread-block clusters (few units and narrow
+ * tables), num_kv_heads * (batch + total_q / (2 * (128 / G))) * (bt_cols * (block_size / 128) * 7 + 24) must be below 2^31, G = num_heads / num_kv_heads
+ * (8 kv heads, 512 sequences of 64 nodes, G = 4: tables of 4.7 million tokens).  The same inputs give the same bits on every call. */
 int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache, int64_t num_blocks,
                    int32_t block_size, const int32_t* block_tables, int64_t bt_row_stride, int32_t bt_cols,
                    const int32_t* cu_seqlens_q, const int32_t* context_lens, const uint64_t* tree_masks, int32_t mask_words,

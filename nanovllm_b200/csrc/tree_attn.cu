@@ -1046,10 +1046,6 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.scale_log2 = scale * 1.4426950408889634f;
   p.scale_abs = scale == 0.f ? std::numeric_limits<float>::denorm_min() : std::fabs(p.scale_log2);
   p.flip = scale < 0.f ? 0x80000000u : 0u;
-  // the longest that the line of key tiles can be (table widths are all that the host knows of the lengths)
-  const double blocks = total_q / (G <= 16 ? 16 / G : 2 * (128 / G)) + batch;
-  const double line = num_kv_heads * blocks * (static_cast<double>(bt_cols) * (block_size / 64) * TcLine::kTilePair + TcLine::kUnitPair);
-  if (line >= 2147483648.0) return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
   const int grid = sm_count();
   if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
   p.pieces = static_cast<TreePieces*>(workspace);
@@ -1076,17 +1072,25 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
     g_launches.fetch_add(1);
     return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn(cluster) launch");
   }
+  // the longest that either kernel's line can be (table widths are all that the host knows of the lengths), in 31 bits
+  const auto line = [&](int block_nodes, int keys, int tile, int unit) {
+    return static_cast<double>(num_kv_heads) * (total_q / block_nodes + static_cast<double>(batch)) *
+           (static_cast<double>(bt_cols) * (block_size / keys) * tile + unit);
+  };
+  const bool small_fits = G <= 16 && line(16 / G, SmLine::kKeys, SmLine::kTilePair, SmLine::kUnitPair) < 2147483648.0;
   // Few nodes to a sequence: tree_small.cu, up to 12 rows on average.  Us of this kernel | that one, calls on end: 256 sequences of
   // 100 .. 2048 tokens at 16/8 heads, 1 node 211 | 179, 4 nodes 216 | 189, 6 nodes (12 rows) 219 | 196, 8 nodes (16 rows) 224 | 215, 12 nodes
   // 231 | 395; 128 of 500 .. 4096 at 32/8, 1 node 205 | 190; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 85 | 73; 64 of
   // 500 .. 3000 at 4/2, 2 .. 10 nodes (12 rows) 31.9 | 32.9; but, with 16 rows, 20 of 300 .. 2000 at 32/8, 4 nodes 31.8 | 34.3, and 64 of
   // 500 .. 3000 at 4/2, 2 .. 14 nodes 34.1 | 38.5.
-  if (G <= 16 && static_cast<long long>(total_q) * G <= 12LL * batch) {
+  if (small_fits && static_cast<long long>(total_q) * G <= 12LL * batch) {
     rc = make_tokens_heads_map(&map_k, k_cache, rows, num_kv_heads, row, 64);
     if (!rc) rc = make_tokens_heads_map(&map_v, v_cache, rows, num_kv_heads, row, 64);
     if (!rc) rc = launch_tree_small(p, map_k, map_v, map_k16, map_v16, grid, static_cast<cudaStream_t>(stream));
     return rc ? rc : launch_tree_join(p, grid, static_cast<cudaStream_t>(stream));
   }
+  if (line(2 * (128 / G), TcLine::kKeys, TcLine::kTilePair, TcLine::kUnitPair) >= 2147483648.0)
+    return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
   rc = tree_configure<false>();
   if (rc) return rc;
   cudaError_t le = launch_early(tree_attn_kernel<false>, grid, kTrThreads, kTrSmem, static_cast<cudaStream_t>(stream), p, map_q, map_k, map_v, map_k16, map_v16);

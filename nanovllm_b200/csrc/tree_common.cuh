@@ -183,6 +183,11 @@ __device__ __forceinline__ void tree_share(const TreeParams& p, int block_nodes,
   }
 }
 
+// Cost of a tile and of a unit in the line of tree_small.cu.
+struct SmLine {
+  static constexpr int kKeys = 64;
+  static constexpr int kTileSplit = 4, kUnitSplit = 18, kTilePair = 4, kUnitPair = 18;
+};
 // Few nodes (tree_small.cu): up to 16 rows to a unit, G <= 16; K/V maps with boxes of 64 and of 16 tokens.
 int launch_tree_small(const TreeParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_k16,
                       const CUtensorMap& map_v16, int ctas, cudaStream_t stream);

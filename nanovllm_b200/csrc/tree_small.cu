@@ -26,12 +26,6 @@ constexpr int kSmItems = 4;
 constexpr int kSmProducer = 8, kSmEpilogue = 9;  // warps: 0-3 and 4-7 consumers, 9-11 epilogue (with 13 warps a scheduler had four, and
 constexpr int kSmThreads = 12 * 32;              // each only 128 registers)
 constexpr int kSmQRow = 256 + 16, kSmQ = 16 * kSmQRow;      // a unit's rows, apart by 4 banks
-// Cost of a tile and of a unit in the line.
-struct SmLine {
-  static constexpr int kKeys = 64;
-  static constexpr int kTileSplit = 4, kUnitSplit = 18, kTilePair = 4, kUnitPair = 18;
-};
-
 static __device__ int g_status_tree_small = 0;
 
 struct SmallItem {

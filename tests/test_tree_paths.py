@@ -53,3 +53,31 @@ def test_attention_scales_that_are_not_positive(path, scale, masks):
     c = dict(case_on(path, 31, masks), scale=scale)
     check_attention(c, run_on(path, on_device(c)))
     status_ok()
+
+
+# ---- how much one call may have ----------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_attention_under_wide_tables():
+    """The limit on a call is of the kernel that it takes: its own blocks of nodes and key tiles, not the other's.  Beyond the limit of the kernel
+    for few nodes the tcgen05 kernel runs, beyond that one's the call is refused."""
+    rng = random.Random(3)
+    c = attention_case(32, 8, [rng.randint(20, 300) for _ in range(40)], [20] * 40, 41)
+    narrow = run_on(LINE, on_device(c))
+    check_attention(c, narrow)
+    args = list(on_device(c))
+    wide = torch.full((40, 40000), 2 ** 31 - 1, dtype=torch.int32, device=DEV)
+    wide[:, :args[5].shape[1]] = args[5]
+    args[5] = wide
+    assert torch.equal(run_on(LINE, args), narrow)
+    c = attention_case(16, 8, [rng.randint(1, 300) for _ in range(100)], [1] * 100, 42)
+    args = list(on_device(c))
+    wide = torch.full((100, 150000), -1, dtype=torch.int32, device=DEV)
+    wide[:, :args[5].shape[1]] = args[5]
+    args[5] = wide
+    check_attention(c, run_on(LINE, args))
+    empty = torch.zeros(1001, dtype=torch.int32, device=DEV)
+    args[0], args[3], args[4] = torch.zeros(1000, 16, 128, dtype=torch.bfloat16, device=DEV), empty, empty[:1000]
+    args[5], args[6] = torch.full((1000, 20000), -1, dtype=torch.int32, device=DEV), torch.zeros(1000, 1, dtype=torch.int64, device=DEV)
+    with pytest.raises(_lib.B200AttnError, match="too many for one call"):
+        nanovllm_b200.tree_attention(*args)
+    status_ok()
