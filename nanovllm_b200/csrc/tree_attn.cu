@@ -29,6 +29,7 @@
 // 128 of 512 .. 4096, 64 nodes, 32/8 324 us (4.1 TB/s, 950 TFLOP/s; 340 where the power cap sets in, up to 400 with L2 flushed between
 // calls): the softmax chain of a tile, about 3100 cycles for both halves against 2048 of tensor work.
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <limits>
 
@@ -139,6 +140,17 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
   const int G = p.G, QT = 128 / p.G;
   // (the join comes in as CTAs of this kernel leave: beside one there is no room)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!kCluster && p.above > 0) {
+    // behind the kernel for few nodes, which as a rule has taken all there is
+    int left = 0;
+#pragma unroll 1
+    for (int i = tid; i < p.batch; i += kTrThreads) left |= min(p.cu_q[i + 1], p.total_q) - max(0, p.cu_q[i]) > p.above;
+    if (!__syncthreads_or(left)) {
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      if (tid == 0) p.pieces->of[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
+    }
+  }
   if (tid == 0) {
     s_abort = 0;
     s_bare = 0;
@@ -777,7 +789,7 @@ constexpr int kTrJoinPieces = 16;             // of 16 dims; 2 of 128
 constexpr int kTrJoinFloats = kTrJoinPieces * (16 * 32 + 64);
 constexpr int kTrJoinWords = kTrMaxCtas / 32;
 
-__global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreeParams p, int ctas) {
+__global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreeParams p, const TreeJoin join_of, int ctas) {
   __shared__ __align__(128) float s_buf[kTrJoinFloats];
   __shared__ float s_weight[kTrJoinPieces][32];
   __shared__ short s_list[kTrMaxCtas + 1];    // places of the unit's pieces
@@ -793,125 +805,138 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
   }
   int loads = 0;                              // phases of the barrier
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int4 piece[kTrJoinWords];                   // nodes of the unit that begins (0: none), how the share begins, that unit
+  // (the second kernel's are looked at along with the first's: mostly there are none)
+  bool second = false;
+  if (join_of.kernels > 1) {
+    int any = 0;
 #pragma unroll
-  for (int w = 0; w < kTrJoinWords; ++w) {
-    const int c = w * 32 + lane;
-    piece[w] = c < ctas ? p.pieces->of[c] : make_int4(0, 0, 0, 0);
+    for (int w = 0; w < kTrJoinWords; ++w)
+      if (w * 32 + lane < ctas) any |= join_of.of[1].pieces->of[w * 32 + lane].x;
+    second = __any_sync(0xffffffffu, any);
   }
-  unsigned heads[kTrJoinWords];
-  int units = 0;
-#pragma unroll
-  for (int w = 0; w < kTrJoinWords; ++w) {
-    heads[w] = __ballot_sync(0xffffffffu, piece[w].x > 0);
-    units += __popc(heads[w]);
-  }
-  // tasks of a unit: 8 groups x 1, 2, 4 or 8 slices of the dims, so that there are about as many as CTAs
-  const int shift = units > 111 ? 0 : units > 55 ? 1 : units > 27 ? 2 : 3;
 #pragma unroll 1
-  for (int task = blockIdx.x; task < units << (3 + shift); task += gridDim.x) {
-    // the unit: the CTA that has its first piece, and how many nodes
-    int k = task >> (3 + shift), c0 = 0, nodes_all = 0;
-    int2 unit = make_int2(0, 0);
-#pragma unroll
-    for (int w = 0; w < kTrJoinWords; ++w) {
-      const unsigned found = __ballot_sync(0xffffffffu, piece[w].x > 0 && __popc(heads[w] & ((1u << lane) - 1)) == k);
-      if (found) {
-        c0 = w * 32 + __ffs(found) - 1;
-        nodes_all = __shfl_sync(0xffffffffu, piece[w].x, __ffs(found) - 1);
-        unit.x = __shfl_sync(0xffffffffu, piece[w].z, __ffs(found) - 1);
-        unit.y = __shfl_sync(0xffffffffu, piece[w].w, __ffs(found) - 1);
-      }
-      k -= __popc(heads[w]);
-    }
-    const int at = task & ((8 << shift) - 1), group = at >> shift, half = group >> 2;
-    const int nodes = half ? nodes_all - QT : min(nodes_all, QT);
-    if ((group & 3) * 32 >= nodes * G) continue;
-    __syncthreads();                          // (the list and the buffer of the task in front have been read)
-    // its pieces: that CTA's second place, then first places up to the unit's last
-    int n = 1;
-    bool open = true;
-    if (tid == 0) s_list[0] = static_cast<short>(2 * c0 + 1);
+  for (int kernel = 0; kernel < (second ? 2 : 1); ++kernel) {
+    const TreeCuts cuts = join_of.of[kernel];
+    int4 piece[kTrJoinWords];                   // nodes of the unit that begins (0: none), how the share begins, that unit
 #pragma unroll
     for (int w = 0; w < kTrJoinWords; ++w) {
       const int c = w * 32 + lane;
-      const unsigned after = __ballot_sync(0xffffffffu, c > c0), last = __ballot_sync(0xffffffffu, piece[w].y == 2) & after;
-      unsigned mine = __ballot_sync(0xffffffffu, piece[w].y != 0) & after;
-      if (last) mine &= last ^ (last - 1);    // up to the first of them
-      if (!open) mine = 0;
-      if (warp == 0 && (mine >> lane) & 1) s_list[n + __popc(mine & ((1u << lane) - 1))] = static_cast<short>(2 * c);
-      n += __popc(mine);
-      open = open && !last;
+      piece[w] = c < ctas ? cuts.pieces->of[c] : make_int4(0, 0, 0, 0);
     }
-    __syncthreads();
-    const int r = (group & 3) * 32 + lane, t = r / G;
-    const int dims_all = 128 >> shift, first_dim = (at & ((1 << shift) - 1)) * dims_all;
-    __nv_bfloat16* const dst = p.out + (static_cast<long long>(unit.x + half * QT + t) * p.H + unit.y * G + (r - t * G)) * 128;
-    // as many dims at a time as let all pieces into the buffer, at least 16
-    const int dims = min(dims_all, n <= 2 ? 128 : n <= 4 ? 64 : n <= 8 ? 32 : 16), stride = dims * 32 + 64;
-#pragma unroll 1
-    for (int dim0 = first_dim; dim0 < first_dim + dims_all; dim0 += dims) {
-      float M = -INFINITY, sum = 0.f, o[16];
-#pragma unroll 1
-      for (int base = 0; base < n; base += kTrJoinPieces) {
-        const int m = min(n - base, kTrJoinPieces);
-        if (loads) __syncthreads();           // the buffer has been read
-        if (tid == 0) mbar_expect_tx(&s_bar, m * stride * 4);
-        __syncwarp();
-        if (tid < m) {
-          // of a piece: its dims, then maxima and sums
-          const float* const from = p.partials + s_list[base + tid] * static_cast<long long>(kTrPartial) + group * kTrGroup;
-          tree_bulk_load(s_buf + tid * stride, from + dim0 * 32, dims * 128, &s_bar);
-          tree_bulk_load(s_buf + tid * stride + dims * 32, from + 128 * 32, 256, &s_bar);
-        }
-        // (a wait that gave up leaves the barriers below complete: nobody leaves)
-        if (!mbar_wait(&s_bar, loads & 1, &s_abort)) atomicExch(&g_status_tree, 1);
-        ++loads;
-        // every warp for itself: the new maximum and sum; the weights are shared out
-        float top = M;
-#pragma unroll 4
-        for (int x = 0; x < m; ++x) top = fmaxf(top, s_buf[x * stride + dims * 32 + lane]);
-        const float ref = top == -INFINITY ? 0.f : top, was = fast_exp2(M - ref);
-        M = top;
-        sum *= was;
-#pragma unroll 4
-        for (int x = 0; x < m; ++x) {
-          const float w = fast_exp2(s_buf[x * stride + dims * 32 + lane] - ref);
-          sum = fmaf(s_buf[x * stride + dims * 32 + 32 + lane], w, sum);
-          if ((x & 3) == warp) s_weight[x][lane] = w;
-        }
-        __syncthreads();
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
-        // a row's dims are a quarter to each warp, up to 16 at a time: two stores then fill a sector (more pieces follow with
-        // 16 dims only)
-        const auto join = [&](auto width) {
-          constexpr int N = decltype(width)::value;
-#pragma unroll 1
-          for (int d = warp * N; d < dims; d += 4 * N) {
+    unsigned heads[kTrJoinWords];
+    int units = 0;
 #pragma unroll
-            for (int i = 0; i < N; ++i) o[i] = N == 4 && base ? o[i] * was : 0.f;
+    for (int w = 0; w < kTrJoinWords; ++w) {
+      heads[w] = __ballot_sync(0xffffffffu, piece[w].x > 0);
+      units += __popc(heads[w]);
+    }
+    // tasks of a unit: 8 groups x 1, 2, 4 or 8 slices of the dims, so that there are about as many as CTAs
+    const int shift = units > 111 ? 0 : units > 55 ? 1 : units > 27 ? 2 : 3;
+#pragma unroll 1
+    for (int task = blockIdx.x; task < units << (3 + shift); task += gridDim.x) {
+      // the unit: the CTA that has its first piece, and how many nodes
+      int k = task >> (3 + shift), c0 = 0, nodes_all = 0;
+      int2 unit = make_int2(0, 0);
+#pragma unroll
+      for (int w = 0; w < kTrJoinWords; ++w) {
+        const unsigned found = __ballot_sync(0xffffffffu, piece[w].x > 0 && __popc(heads[w] & ((1u << lane) - 1)) == k);
+        if (found) {
+          c0 = w * 32 + __ffs(found) - 1;
+          nodes_all = __shfl_sync(0xffffffffu, piece[w].x, __ffs(found) - 1);
+          unit.x = __shfl_sync(0xffffffffu, piece[w].z, __ffs(found) - 1);
+          unit.y = __shfl_sync(0xffffffffu, piece[w].w, __ffs(found) - 1);
+        }
+        k -= __popc(heads[w]);
+      }
+      const int at = task & ((8 << shift) - 1), group = at >> shift, half = group >> 2;
+      const int nodes = half ? nodes_all - QT : min(nodes_all, QT);
+      if ((group & 3) * 32 >= nodes * G) continue;
+      __syncthreads();                          // (the list and the buffer of the task in front have been read)
+      // its pieces: that CTA's second place, then first places up to the unit's last
+      int n = 1;
+      bool open = true;
+      if (tid == 0) s_list[0] = static_cast<short>(2 * c0 + 1);
+#pragma unroll
+      for (int w = 0; w < kTrJoinWords; ++w) {
+        const int c = w * 32 + lane;
+        const unsigned after = __ballot_sync(0xffffffffu, c > c0), last = __ballot_sync(0xffffffffu, piece[w].y == 2) & after;
+        unsigned mine = __ballot_sync(0xffffffffu, piece[w].y != 0) & after;
+        if (last) mine &= last ^ (last - 1);    // up to the first of them
+        if (!open) mine = 0;
+        if (warp == 0 && (mine >> lane) & 1) s_list[n + __popc(mine & ((1u << lane) - 1))] = static_cast<short>(2 * c);
+        n += __popc(mine);
+        open = open && !last;
+      }
+      __syncthreads();
+      const int r = (group & 3) * 32 + lane, t = r / G;
+      const int dims_all = 128 >> shift, first_dim = (at & ((1 << shift) - 1)) * dims_all;
+      __nv_bfloat16* const dst = p.out + (static_cast<long long>(unit.x + half * QT + t) * p.H + unit.y * G + (r - t * G)) * 128;
+      // as many dims at a time as let all pieces into the buffer, at least 16
+      const int dims = min(dims_all, n <= 2 ? 128 : n <= 4 ? 64 : n <= 8 ? 32 : 16), stride = dims * 32 + 64;
+#pragma unroll 1
+      for (int dim0 = first_dim; dim0 < first_dim + dims_all; dim0 += dims) {
+        float M = -INFINITY, sum = 0.f, o[16];
+#pragma unroll 1
+        for (int base = 0; base < n; base += kTrJoinPieces) {
+          const int m = min(n - base, kTrJoinPieces);
+          if (loads) __syncthreads();           // the buffer has been read
+          if (tid == 0) mbar_expect_tx(&s_bar, m * stride * 4);
+          __syncwarp();
+          if (tid < m) {
+            // of a piece: its dims, then maxima and sums
+            const float* const from = cuts.partials + s_list[base + tid] * static_cast<long long>(cuts.stride) + group * kTrGroup;
+            tree_bulk_load(s_buf + tid * stride, from + dim0 * 32, dims * 128, &s_bar);
+            tree_bulk_load(s_buf + tid * stride + dims * 32, from + 128 * 32, 256, &s_bar);
+          }
+          // (a wait that gave up leaves the barriers below complete: nobody leaves)
+          if (!mbar_wait(&s_bar, loads & 1, &s_abort)) atomicExch(&g_status_tree, 1);
+          ++loads;
+          // every warp for itself: the new maximum and sum; the weights are shared out
+          float top = M;
+#pragma unroll 4
+          for (int x = 0; x < m; ++x) top = fmaxf(top, s_buf[x * stride + dims * 32 + lane]);
+          const float ref = top == -INFINITY ? 0.f : top, was = fast_exp2(M - ref);
+          M = top;
+          sum *= was;
+#pragma unroll 4
+          for (int x = 0; x < m; ++x) {
+            const float w = fast_exp2(s_buf[x * stride + dims * 32 + lane] - ref);
+            sum = fmaf(s_buf[x * stride + dims * 32 + 32 + lane], w, sum);
+            if ((x & 3) == warp) s_weight[x][lane] = w;
+          }
+          __syncthreads();
+          const float inv = sum > 0.f ? 1.f / sum : 0.f;
+          // a row's dims are a quarter to each warp, up to 16 at a time: two stores then fill a sector (more pieces follow with
+          // 16 dims only)
+          const auto join = [&](auto width) {
+            constexpr int N = decltype(width)::value;
+#pragma unroll 1
+            for (int d = warp * N; d < dims; d += 4 * N) {
+#pragma unroll
+              for (int i = 0; i < N; ++i) o[i] = N == 4 && base ? o[i] * was : 0.f;
 #pragma unroll 2
-            for (int x = 0; x < m; ++x) {
-              const float w = s_weight[x][lane];
+              for (int x = 0; x < m; ++x) {
+                const float w = s_weight[x][lane];
 #pragma unroll
-              for (int i = 0; i < N; ++i) o[i] = fmaf(s_buf[x * stride + (d + i) * 32 + lane], w, o[i]);
-            }
-            if (base + m == n && r < nodes * G) {
+                for (int i = 0; i < N; ++i) o[i] = fmaf(s_buf[x * stride + (d + i) * 32 + lane], w, o[i]);
+              }
+              if (base + m == n && r < nodes * G) {
 #pragma unroll
-              for (int i = 0; i < N; i += 8) {
-                const uint2 a = make_uint2(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv));
-                if constexpr (N == 4)
-                  *reinterpret_cast<uint2*>(dst + dim0 + d) = a;
-                else
-                  *reinterpret_cast<uint4*>(dst + dim0 + d + i) =
-                      make_uint4(a.x, a.y, pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                for (int i = 0; i < N; i += 8) {
+                  const uint2 a = make_uint2(pack_bf16(o[i] * inv, o[i + 1] * inv), pack_bf16(o[i + 2] * inv, o[i + 3] * inv));
+                  if constexpr (N == 4)
+                    *reinterpret_cast<uint2*>(dst + dim0 + d) = a;
+                  else
+                    *reinterpret_cast<uint4*>(dst + dim0 + d + i) =
+                        make_uint4(a.x, a.y, pack_bf16(o[i + 4] * inv, o[i + 5] * inv), pack_bf16(o[i + 6] * inv, o[i + 7] * inv));
+                }
               }
             }
-          }
-        };
-        if (dims == 16) join(std::integral_constant<int, 4>{});
-        else if (dims == 32) join(std::integral_constant<int, 8>{});
-        else join(std::integral_constant<int, 16>{});
+          };
+          if (dims == 16) join(std::integral_constant<int, 4>{});
+          else if (dims == 32) join(std::integral_constant<int, 8>{});
+          else join(std::integral_constant<int, 16>{});
+        }
       }
     }
   }
@@ -927,6 +952,11 @@ constexpr size_t kTrSmem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTil
 // (What clusters lose, they lose where lengths differ; wider tables make that worse: 4 of 300 .. 8000 lost 8 us, 6 of them 5.)
 constexpr int kTrClusterSizes = 3;
 constexpr int kTrClusterTiles[kTrClusterSizes] = {128, 40, 32};
+// Blocks of 16 / G nodes that a sequence may have in the kernel for few nodes, which reads its keys once for each.  Us with 1 | 2 | 4 | without a limit, calls on end
+// in a graph at 16/8 heads: 48 sequences of 1 node and 16 of 16 (2 blocks), all of 500 .. 3000 tokens 95 | 110 | 110 | 107; 56 of 1 and 8 of 32
+// (4 blocks) on 4000 107 | 107 | 124 | 122; 200 of 2 and 56 of 18 (3), 100 .. 2048 198 | 198 | 274 | 273; 64 of 1 and one of 256 (32) on 40000 168 | 168 | 168 | 642;
+// 64 of 2 .. 10 (up to 2) at 4/2 heads 44.7 | 35.5 | 35.5 | 32.7.  (What is more than without it is the launch that finds nothing to do: 3 us.)
+constexpr int kSmMostBlocks = 2;
 
 template <bool kCluster>
 static int tree_configure() {
@@ -965,13 +995,13 @@ static int tree_clusters_on_chip(int i) {
   return n;
 }
 
-// Workspace: the pieces' records, then two places of partial results per CTA.
+// Workspace: the records of this kernel's pieces and of those of tree_small.cu, then two places of partial results per CTA for each.
 constexpr int64_t kTrPiecesBytes = (sizeof(TreePieces) + 255) / 256 * 256;
-static int64_t tree_workspace(int ctas) { return kTrPiecesBytes + static_cast<int64_t>(ctas) * 2 * kTrPartial * 4; }
+static int64_t tree_workspace(int ctas) { return 2 * kTrPiecesBytes + static_cast<int64_t>(ctas) * 2 * (kTrPartial + kSmPartial) * 4; }
 
-int launch_tree_join(const TreeParams& p, int ctas, cudaStream_t stream) {
+int launch_tree_join(const TreeParams& p, const TreeJoin& join, int ctas, cudaStream_t stream) {
   if (ctas < 2) return kOk;
-  const cudaError_t le = launch_early(tree_join_kernel, ctas * kTrJoinCtas, kTrJoinThreads, 0, stream, p, ctas);
+  const cudaError_t le = launch_early(tree_join_kernel, ctas * kTrJoinCtas, kTrJoinThreads, 0, stream, p, join, ctas);
   g_launches.fetch_add(1);
   return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn join launch");
 }
@@ -1048,9 +1078,12 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.flip = scale < 0.f ? 0x80000000u : 0u;
   const int grid = sm_count();
   if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
-  p.pieces = static_cast<TreePieces*>(workspace);
-  p.partials = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTrPiecesBytes);
-  CUtensorMap map_q, map_k, map_v, map_k16, map_v16;
+  char* const ws = static_cast<char*>(workspace);
+  p.above = 0;
+  p.upto = INT_MAX;
+  p.pieces = reinterpret_cast<TreePieces*>(ws);
+  p.partials = reinterpret_cast<float*>(ws + 2 * kTrPiecesBytes);
+  CUtensorMap map_q, map_k, map_v, map_k16, map_v16, map_k64, map_v64;
   const uint64_t rows = static_cast<uint64_t>(num_blocks) * block_size, row = static_cast<uint64_t>(num_kv_heads) * 128;
   int rc = make_tokens_heads_map(&map_q, q, static_cast<uint64_t>(total_q), num_heads, static_cast<uint64_t>(q_row_stride), 128 / G, G);
   if (!rc) rc = make_tokens_heads_map(&map_k, k_cache, rows, num_kv_heads, row, kTrKv);
@@ -1077,25 +1110,36 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
     return static_cast<double>(num_kv_heads) * (total_q / block_nodes + static_cast<double>(batch)) *
            (static_cast<double>(bt_cols) * (block_size / keys) * tile + unit);
   };
-  const bool small_fits = G <= 16 && line(16 / G, SmLine::kKeys, SmLine::kTilePair, SmLine::kUnitPair) < 2147483648.0;
-  // Few nodes to a sequence: tree_small.cu, up to 12 rows on average.  Us of this kernel | that one, calls on end: 256 sequences of
-  // 100 .. 2048 tokens at 16/8 heads, 1 node 211 | 179, 4 nodes 216 | 189, 6 nodes (12 rows) 219 | 196, 8 nodes (16 rows) 224 | 215, 12 nodes
-  // 231 | 395; 128 of 500 .. 4096 at 32/8, 1 node 205 | 190; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 85 | 73; 64 of
-  // 500 .. 3000 at 4/2, 2 .. 10 nodes (12 rows) 31.9 | 32.9; but, with 16 rows, 20 of 300 .. 2000 at 32/8, 4 nodes 31.8 | 34.3, and 64 of
-  // 500 .. 3000 at 4/2, 2 .. 14 nodes 34.1 | 38.5.
-  if (small_fits && static_cast<long long>(total_q) * G <= 12LL * batch) {
-    rc = make_tokens_heads_map(&map_k, k_cache, rows, num_kv_heads, row, 64);
-    if (!rc) rc = make_tokens_heads_map(&map_v, v_cache, rows, num_kv_heads, row, 64);
-    if (!rc) rc = launch_tree_small(p, map_k, map_v, map_k16, map_v16, grid, static_cast<cudaStream_t>(stream));
-    return rc ? rc : launch_tree_join(p, grid, static_cast<cudaStream_t>(stream));
-  }
   if (line(2 * (128 / G), TcLine::kKeys, TcLine::kTilePair, TcLine::kUnitPair) >= 2147483648.0)
     return set_error(kErrBadShape, "tree_attn: %d sequences with tables of %d blocks are too many for one call", batch, bt_cols);
-  rc = tree_configure<false>();
-  if (rc) return rc;
-  cudaError_t le = launch_early(tree_attn_kernel<false>, grid, kTrThreads, kTrSmem, static_cast<cudaStream_t>(stream), p, map_q, map_k, map_v, map_k16, map_v16);
-  g_launches.fetch_add(1);
-  rc = check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn launch");
-  if (rc) return rc;
-  return launch_tree_join(p, grid, static_cast<cudaStream_t>(stream));
+  const bool small_fits = G <= 16 && line(16 / G, SmLine::kKeys, SmLine::kTilePair, SmLine::kUnitPair) < 2147483648.0;
+  TreeJoin join = {{{p.pieces, p.partials, kTrPartial}, {}}, 1};
+  // Few nodes to a sequence: tree_small.cu, up to 12 rows on average.  Us of this kernel | that one with the launch behind it, calls on end in a graph:
+  // 256 sequences of 100 .. 2048 tokens at 16/8 heads, 1 node 227 | 181, 4 nodes 233 | 191, 6 nodes (12 rows) 232 | 202, 8 nodes (16 rows) 233 | 218,
+  // 12 nodes 238 | 402; 128 of 500 .. 4096 at 32/8, 1 node 215 | 193; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 98 | 77; 64 of 500 .. 3000 at
+  // 4/2, 3 nodes 33.5 | 31.6, 2 .. 10 nodes (12 rows) 33.1 | 36.0, 2 .. 14 nodes (16 rows) 32.8 | 39.2; 20 of 300 .. 2000 at 32/8, 3 nodes (12 rows) 30.0 | 31.5,
+  // 4 nodes (16 rows) 30.1 | 34.2.  (Lengths are not known here, so short calls pay up to 3 us for what long ones gain.)
+  // A sequence has its keys read once for every 16 / G of its nodes there, so those with more than kSmMostBlocks times that are left to this kernel, in
+  // a launch behind that one (which leaves at once where there are none).
+  if (small_fits && static_cast<long long>(total_q) * G <= 12LL * batch) {
+    rc = make_tokens_heads_map(&map_k64, k_cache, rows, num_kv_heads, row, 64);
+    if (!rc) rc = make_tokens_heads_map(&map_v64, v_cache, rows, num_kv_heads, row, 64);
+    TreeParams few = p;
+    few.upto = kSmMostBlocks * (16 / G);
+    few.pieces = reinterpret_cast<TreePieces*>(ws + kTrPiecesBytes);
+    few.partials = p.partials + static_cast<int64_t>(grid) * 2 * kTrPartial;
+    if (!rc) rc = launch_tree_small(few, map_k64, map_v64, map_k16, map_v16, grid, static_cast<cudaStream_t>(stream));
+    if (rc) return rc;
+    p.above = few.upto;
+    join = {{{few.pieces, few.partials, kSmPartial}, join.of[0]}, total_q > p.above ? 2 : 1};
+  }
+  if (total_q > p.above) {
+    rc = tree_configure<false>();
+    if (rc) return rc;
+    const cudaError_t le = launch_early(tree_attn_kernel<false>, grid, kTrThreads, kTrSmem, static_cast<cudaStream_t>(stream), p, map_q, map_k, map_v, map_k16, map_v16);
+    g_launches.fetch_add(1);
+    rc = check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn launch");
+    if (rc) return rc;
+  }
+  return launch_tree_join(p, join, grid, static_cast<cudaStream_t>(stream));
 }

@@ -19,6 +19,7 @@ struct TreeParams {
   const uint32_t* masks;             // (total_q, mask_words) 32-bit words; nullptr: each node sees those before it and itself
   int mask_words;                    // 32-bit words of a row
   int batch, total_q, H, Hkv, G;
+  int above, upto;                   // sequences with more than `above` and at most `upto` nodes are this launch's
   float scale_log2;
   // The tcgen05 kernel takes the maximum of unscaled scores, which wants a positive scale: it is scale_abs (of 0 the least number
   // above, so that -inf stays -inf), and `flip`, the sign bit of a negative one, goes over the scores.
@@ -60,6 +61,7 @@ struct TreePieces {
 // move whole lines with a row per lane.
 constexpr int kTrGroup = 130 * 32;
 constexpr int kTrPartial = 8 * kTrGroup;      // floats
+constexpr int kSmPartial = kTrGroup;          // (tree_small.cu has at most 16 rows)
 
 // One sequence as the line sees it.
 struct TreeSeq {
@@ -71,6 +73,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int block_nodes
   TreeSeq s;
   s.q_begin = max(0, min(p.cu_q[i], p.total_q));
   s.nodes = max(0, min(p.cu_q[i + 1], p.total_q) - s.q_begin);
+  if (s.nodes <= p.above || s.nodes > p.upto) s.nodes = 0;
   s.Lk = max(0, min(p.context_lens[i], p.bt_cols * p.block_size));
   s.tiles = (s.Lk + L::kKeys - 1) / L::kKeys;
   s.blocks = s.tiles > 0 ? (s.nodes + block_nodes - 1) / block_nodes : 0;
@@ -191,7 +194,16 @@ struct SmLine {
 // Few nodes (tree_small.cu): up to 16 rows to a unit, G <= 16; K/V maps with boxes of 64 and of 16 tokens.
 int launch_tree_small(const TreeParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_k16,
                       const CUtensorMap& map_v16, int ctas, cudaStream_t stream);
-// Joins the pieces of cut units (tree_attn.cu): to be launched behind a kernel of `ctas` CTAs that wrote p.pieces.
-int launch_tree_join(const TreeParams& p, int ctas, cudaStream_t stream);
+// What a kernel of `ctas` CTAs leaves for the join (tree_attn.cu): records, partial results, floats from one of these to the next.
+struct TreeCuts {
+  const TreePieces* pieces;
+  const float* partials;
+  int stride;
+};
+struct TreeJoin {
+  TreeCuts of[2];
+  int kernels;
+};
+int launch_tree_join(const TreeParams& p, const TreeJoin& join, int ctas, cudaStream_t stream);
 
 }  // namespace b200

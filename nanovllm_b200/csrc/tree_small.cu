@@ -439,7 +439,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
         *reinterpret_cast<uint2*>(p.out + (static_cast<long long>(it.q_row + t) * p.H + it.h * G + (r - t * G)) * 128 + lane * 4) =
             make_uint2(pack_bf16(o4.x * inv, o4.y * inv), pack_bf16(o4.z * inv, o4.w * inv));
       } else {
-        float* const part = p.partials + static_cast<long long>(it.partial) * kTrPartial + r;
+        float* const part = p.partials + static_cast<long long>(it.partial) * kSmPartial + r;
         part[(lane * 4) * 32] = o4.x;
         part[(lane * 4 + 1) * 32] = o4.y;
         part[(lane * 4 + 2) * 32] = o4.z;

@@ -1,5 +1,6 @@
-"""Tree attention by the kernel that a call takes: clusters (one launch), the tcgen05 line and the kernel for few nodes (more:
-units that the line cuts are joined by a launch of their own).  Inputs, oracle and tolerance are those of test_tree_decode."""
+"""Tree attention by the kernel that a call takes: clusters (one launch), the tcgen05 line (two: units that it cuts are joined by a
+launch of their own), and the kernel for few nodes (three: the tcgen05 line behind it takes the sequences with many nodes).
+Inputs, oracle and tolerance are those of test_tree_decode."""
 import random
 
 import pytest
@@ -24,10 +25,10 @@ def on_device(c):
 
 
 def run_on(path, args):
-    """The call's result, and a look whether it took that kernel: a cluster is one launch, the others come with a join."""
+    """The call's result, and a look whether it took that kernel."""
     before = _lib.load().b200_launch_count()
     out = nanovllm_b200.tree_attention(*args)
-    assert (_lib.load().b200_launch_count() - before == 1) == (path == CLUSTER)
+    assert _lib.load().b200_launch_count() - before == {CLUSTER: 1, LINE: 2, FEW: 3}[path]
     return out
 
 
@@ -80,4 +81,38 @@ def test_attention_under_wide_tables():
     args[5], args[6] = torch.full((1000, 20000), -1, dtype=torch.int32, device=DEV), torch.zeros(1000, 1, dtype=torch.int64, device=DEV)
     with pytest.raises(_lib.B200AttnError, match="too many for one call"):
         nanovllm_b200.tree_attention(*args)
+    status_ok()
+
+
+# ---- batches with few nodes to most sequences -----------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,hkv,limit", [(16, 8, 16), (32, 8, 8), (5, 1, 6), (16, 1, 2), (3, 3, 32), (28, 4, 4)])
+@pytest.mark.parametrize("masks", ["tree", "chain", "any"])
+def test_attention_large_trees_among_small_ones(H, hkv, limit, masks):
+    """Sequences with more than `limit` nodes (twice what a unit of 16 rows holds) go to the other kernel, those with as many do not: each
+    reads its keys a few times, whatever the mean.  Among both kinds some have no context or fewer tokens than nodes."""
+    rng = random.Random(limit)
+    ctx = [1, 300, 65, 700, 0, 257, 40, -1, 512, 33, 128, 64]
+    nodes = [1, limit, limit + 1, 256, limit + 3, limit, 2, 1, 2 * limit + 1, limit + 1, 1, 0]
+    while sum(nodes) * (H // hkv) > 12 * len(ctx) or len(ctx) * hkv <= 74:
+        ctx.append(rng.choice((1, 16, 90, 200)))
+        nodes.append(rng.choice((0, 1)))
+    c = attention_case(H, hkv, ctx, nodes, seed=H, masks=masks, extra_rows=1)
+    c["total"] -= 1                                     # (rows behind the last sequence would count in the mean)
+    c["q"], c["masks"] = c["q"][:-1], c["masks"] if c["masks"] is None else c["masks"][:-1]
+    out = run_on(FEW, on_device(c))
+    check_attention(c, out)
+    assert all(torch.equal(out, run_on(FEW, on_device(c))) for _ in range(3))
+    status_ok()
+
+
+@pytest.mark.gpu
+def test_attention_large_trees_alone_and_long():
+    """One tree on a long context among sequences without nodes (padded rows of a graph) and with one; no sequence can have many."""
+    c = attention_case(16, 8, [9000] + [0] * 20 + [200] * 40, [60] + [0] * 20 + [1] * 40, 51)
+    check_attention(c, run_on(FEW, on_device(c)))
+    c = attention_case(16, 8, [9000] + [3] * 49, [250] + [0] * 49, 52)
+    check_attention(c, run_on(FEW, on_device(c)))
+    c = attention_case(16, 8, [300] * 12, [1] * 12, 53)            # (12 nodes in all: two launches)
+    check_attention(c, run_on(LINE, on_device(c)))
     status_ok()
