@@ -279,8 +279,8 @@ int b200_accept_tree(const int64_t* draft_tokens, const int64_t* target_tokens, 
 
 /* The accepted nodes' rows to their places, in all planes of a cache (K and V of every layer; plane_stride_bytes apart,
  * each num_blocks * block_size rows of row_bytes): the row of position start_lens[i] + path[i][k] goes to start_lens[i] + k
- * for k < accepted[i], path (batch, path_cols) contiguous.  path ascends; entries below their place (path[i][k] < k) are not
- * moved, nor is anything from or to a position without a block of the cache, or with a negative start length.  Pure byte copy.  Sequences must not share
+ * for k < accepted[i], path (batch, path_cols) contiguous.  path ascends, from the root on (a path of one column is the root alone: nothing
+ * is moved); entries below their place (path[i][k] < k) are not moved, nor is anything from or to a position without a block of the cache, or with a negative start length.  Pure byte copy.  Sequences must not share
  * the blocks behind their start lengths.  batch is at most 65535. */
 int b200_compact_kvcache(void* cache, int32_t planes, int64_t plane_stride_bytes, int64_t row_bytes, int64_t num_blocks,
                          int32_t block_size, const int32_t* path, int32_t path_cols, const int32_t* accepted,
