@@ -45,7 +45,8 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr, uint32_t
 
 // Instruction descriptor for kind::f16 with bf16 inputs and fp32 accumulation.
 //  [4,6) D format 1 = f32 | [7,10) A format 1 = bf16 | [10,13) B format 1 = bf16
-//  bit 15 A major, bit 16 B major (0 = K-major, 1 = MN-major) | [17,23) N >> 3 | [24,29) M >> 4
+//  bit 13 negate A, bit 14 negate B | bit 15 A major, bit 16 B major (0 = K-major, 1 = MN-major) | [17,23) N >> 3 | [24,29) M >> 4
+constexpr uint32_t kIdescNegateA = 1u << 13;
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int m, int n, bool a_mn_major, bool b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(a_mn_major) << 15) |
          (static_cast<uint32_t>(b_mn_major) << 16) | (static_cast<uint32_t>(n >> 3) << 17) |

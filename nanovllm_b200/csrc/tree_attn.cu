@@ -331,7 +331,8 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
       }
     } else if (warp == 1 && lane == 0) {
       // ================================ S = Q K^T ================================
-      constexpr uint32_t idesc_qk = tc::idesc_bf16_f32(128, 128, false, false);
+      // (the sign of a negative scale: in the softmax, a pass of its own over S, it cost every call up to 1 %)
+      const uint32_t idesc_qk = tc::idesc_bf16_f32(128, 128, false, false) | p.negate;
       constexpr uint32_t desc_hi = tc::smem_desc_sw128_hi(1024);
       const uint32_t q_lo = tc::smem_desc_sw128_lo(smem_u32(sQ), 16), k_lo = tc::smem_desc_sw128_lo(smem_u32(sK), 16);
       int n_item = 0, q_use = 0, k_at = 0, k_ph = 0, n_step = 0;
@@ -469,19 +470,6 @@ tree_attn_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, 
         const int key0 = (it.t0 + (it.split ? 2 * j + mine : j)) * kTrKv;
         if (active) {
           tc::fence_after_sync();
-          if (p.flip) {
-            // a negative scale: scores of the other sign over S (a pass of its own: in the one below it cost all calls 0.5 us)
-#pragma unroll 1
-            for (int cch = 0; cch < 8; ++cch) {
-              uint32_t v[16];
-              tc::ld_32x32b_x16(tmem_s + cch * 16, v);
-              tc::wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] ^= p.flip;
-              tc::st_32x32b_x16(tmem_s + cch * 16, v);
-            }
-            tc::wait_st();
-          }
           if (key0 + kTrKv > min(it.first, it.Lk)) {
             // the tile reaches the nodes: masked scores go back over S first (rolled: the hot code stays short)
 #pragma unroll 1
@@ -1075,7 +1063,7 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   p.G = G;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.scale_abs = scale == 0.f ? std::numeric_limits<float>::denorm_min() : std::fabs(p.scale_log2);
-  p.flip = scale < 0.f ? 0x80000000u : 0u;
+  p.negate = scale < 0.f ? tc::kIdescNegateA : 0u;
   const int grid = sm_count();
   if (grid > kTrMaxCtas) return set_error(kErrDevice, "tree_attn: more than %d multiprocessors", kTrMaxCtas);
   char* const ws = static_cast<char*>(workspace);

@@ -22,9 +22,9 @@ struct TreeParams {
   int above, upto;                   // sequences with more than `above` and at most `upto` nodes are this launch's
   float scale_log2;
   // The tcgen05 kernel takes the maximum of unscaled scores, which wants a positive scale: it is scale_abs (of 0 the least number
-  // above, so that -inf stays -inf), and `flip`, the sign bit of a negative one, goes over the scores.
+  // above, so that -inf stays -inf), and of a negative one `negate`, a bit of the instruction descriptor, turns Q.
   float scale_abs;
-  uint32_t flip;
+  uint32_t negate;
   int cluster_log;                   // where a cluster has a unit: log2 of its CTAs
   struct TreePieces* pieces;         // records of cut units
   float* partials;                   // [2 * CTAs] partial results
