@@ -777,6 +777,8 @@ constexpr int kTrJoinPieces = 16;             // of 16 dims; 2 of 128
 constexpr int kTrJoinFloats = kTrJoinPieces * (16 * 32 + 64);
 constexpr int kTrJoinWords = kTrMaxCtas / 32;
 
+// kTwo: of two kernels (a form of its own: as one, with 128 registers for 95, it cost 128 trees of 64 nodes 2.4 of 341 us).
+template <bool kTwo>
 __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreeParams p, const TreeJoin join_of, int ctas) {
   __shared__ __align__(128) float s_buf[kTrJoinFloats];
   __shared__ float s_weight[kTrJoinPieces][32];
@@ -795,7 +797,7 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // (the second kernel's are looked at along with the first's: mostly there are none)
   bool second = false;
-  if (join_of.kernels > 1) {
+  if constexpr (kTwo) {
     int any = 0;
 #pragma unroll
     for (int w = 0; w < kTrJoinWords; ++w)
@@ -803,8 +805,9 @@ __global__ void __launch_bounds__(kTrJoinThreads) tree_join_kernel(const TreePar
     second = __any_sync(0xffffffffu, any);
   }
 #pragma unroll 1
-  for (int kernel = 0; kernel < (second ? 2 : 1); ++kernel) {
-    const TreeCuts cuts = join_of.of[kernel];
+  for (int kernel = 0; kernel < (kTwo && second ? 2 : 1); ++kernel) {
+    const TreeCuts cuts = {kTwo && kernel ? join_of.of[1].pieces : join_of.of[0].pieces, kTwo && kernel ? join_of.of[1].partials : join_of.of[0].partials,
+                           kTwo && kernel ? join_of.of[1].stride : join_of.of[0].stride};
     int4 piece[kTrJoinWords];                   // nodes of the unit that begins (0: none), how the share begins, that unit
 #pragma unroll
     for (int w = 0; w < kTrJoinWords; ++w) {
@@ -940,10 +943,10 @@ constexpr size_t kTrSmem = static_cast<size_t>(2 + kTrRingK + kTrRingV) * kTrTil
 // (What clusters lose, they lose where lengths differ; wider tables make that worse: 4 of 300 .. 8000 lost 8 us, 6 of them 5.)
 constexpr int kTrClusterSizes = 3;
 constexpr int kTrClusterTiles[kTrClusterSizes] = {128, 40, 32};
-// Blocks of 16 / G nodes that a sequence may have in the kernel for few nodes, which reads its keys once for each.  Us with 1 | 2 | 4 | without a limit, calls on end
-// in a graph at 16/8 heads: 48 sequences of 1 node and 16 of 16 (2 blocks), all of 500 .. 3000 tokens 95 | 110 | 110 | 107; 56 of 1 and 8 of 32
-// (4 blocks) on 4000 107 | 107 | 124 | 122; 200 of 2 and 56 of 18 (3), 100 .. 2048 198 | 198 | 274 | 273; 64 of 1 and one of 256 (32) on 40000 168 | 168 | 168 | 642;
-// 64 of 2 .. 10 (up to 2) at 4/2 heads 44.7 | 35.5 | 35.5 | 32.7.  (What is more than without it is the launch that finds nothing to do: 3 us.)
+// Blocks of 16 / G nodes that a sequence may have in the kernel for few nodes, which reads its keys once for each.  Us with 1 | 2 | 4 | without a limit (and
+// the launch behind it), calls on end in a graph at 16/8 heads: 48 sequences of 1 node and 16 of 16 (2 blocks), all of 500 .. 3000 tokens 96 | 111 | 112 | 113; 56
+// of 1 and 8 of 32 (4 blocks) on 4000 110 | 110 | 127 | 134; 200 of 2 and 56 of 18 (3), 100 .. 2048 200 | 200 | 282 | 279; 64 of 1 and one of 256 (32) on
+// 40000 166 | 167 | 167 | 660; 256 of 4 (1) 189 | 189 | 188 | 186; 64 of 2 .. 10 (up to 2) at 4/2 heads 45.5 | 36.0 | 35.7 | 33.3.
 constexpr int kSmMostBlocks = 2;
 
 template <bool kCluster>
@@ -989,7 +992,7 @@ static int64_t tree_workspace(int ctas) { return 2 * kTrPiecesBytes + static_cas
 
 int launch_tree_join(const TreeParams& p, const TreeJoin& join, int ctas, cudaStream_t stream) {
   if (ctas < 2) return kOk;
-  const cudaError_t le = launch_early(tree_join_kernel, ctas * kTrJoinCtas, kTrJoinThreads, 0, stream, p, join, ctas);
+  const cudaError_t le = launch_early(join.kernels > 1 ? tree_join_kernel<true> : tree_join_kernel<false>, ctas * kTrJoinCtas, kTrJoinThreads, 0, stream, p, join, ctas);
   g_launches.fetch_add(1);
   return check_cuda(le != cudaSuccess ? le : cudaGetLastError(), "tree_attn join launch");
 }
@@ -1103,10 +1106,10 @@ extern "C" int b200_tree_attn(const void* q, int64_t q_row_stride, const void* k
   const bool small_fits = G <= 16 && line(16 / G, SmLine::kKeys, SmLine::kTilePair, SmLine::kUnitPair) < 2147483648.0;
   TreeJoin join = {{{p.pieces, p.partials, kTrPartial}, {}}, 1};
   // Few nodes to a sequence: tree_small.cu, up to 12 rows on average.  Us of this kernel | that one with the launch behind it, calls on end in a graph:
-  // 256 sequences of 100 .. 2048 tokens at 16/8 heads, 1 node 227 | 181, 4 nodes 233 | 191, 6 nodes (12 rows) 232 | 202, 8 nodes (16 rows) 233 | 218,
-  // 12 nodes 238 | 402; 128 of 500 .. 4096 at 32/8, 1 node 215 | 193; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 98 | 77; 64 of 500 .. 3000 at
-  // 4/2, 3 nodes 33.5 | 31.6, 2 .. 10 nodes (12 rows) 33.1 | 36.0, 2 .. 14 nodes (16 rows) 32.8 | 39.2; 20 of 300 .. 2000 at 32/8, 3 nodes (12 rows) 30.0 | 31.5,
-  // 4 nodes (16 rows) 30.1 | 34.2.  (Lengths are not known here, so short calls pay up to 3 us for what long ones gain.)
+  // 256 sequences of 100 .. 2048 tokens at 16/8 heads, 1 node 213 | 180, 4 nodes 212 to 226 | 190, 6 nodes (12 rows) 219 to 229 | 200, 8 nodes (16 rows)
+  // 221 to 231 | 217, 12 nodes 238 | 398; 128 of 500 .. 4096 at 32/8, 1 node 209 | 192; 256 of 100 .. 1000 at 8/4, 3 .. 9 nodes (12 rows) 106 | 78; 64 of
+  // 500 .. 3000 at 4/2, 3 nodes 32.2 | 30.5, 2 .. 10 nodes (12 rows) 32.2 | 35.4, 2 .. 14 nodes (16 rows) 31.8 | 38.5; 20 of 300 .. 2000 at 32/8, 3 nodes
+  // (12 rows) 29.7 | 30.9, 4 nodes (16 rows) 29.9 | 33.4.  (Lengths are not known here, so some short calls pay 1 to 3 us for what long ones gain.)
   // A sequence has its keys read once for every 16 / G of its nodes there, so those with more than kSmMostBlocks times that are left to this kernel, in
   // a launch behind that one (which leaves at once where there are none).
   if (small_fits && static_cast<long long>(total_q) * G <= 12LL * batch) {
