@@ -2,8 +2,9 @@
 // are already in the cache behind its context.  A node sees the context, and of the nodes those that its mask names.
 //
 // Bytes: K and V once per (sequence, kv head), whatever the number of nodes: rows = nodes x query heads of the group share them.
-// At 8 rows that is 8 flops a byte, at 256 it is 256, where tensor throughput and HBM balance.  tcgen05 carries all of it: a tile
-// of 128 rows costs the tensor core the same however few of them are nodes, and that is less time than its bytes take.
+// At 8 rows that is 8 flops a byte, at 256 it is 256, where tensor throughput and HBM balance.  A tile of 128 rows costs tcgen05 the
+// same however few of them are nodes, and that is less time than its bytes take (but power: batches with few nodes to a sequence
+// go to tree_small.cu, which leaves this kernel the large trees among them).
 //
 // One persistent CTA per SM.  A unit is (sequence, block of up to 2 * QT nodes, kv head), QT = 128 / G.  All units' key tiles (128
 // keys) stand in one line, which is cut into equal shares, one per CTA; a unit that a cut runs through leaves partial
@@ -26,8 +27,8 @@
 // Calls on end in a graph (with the join): 1 sequence of 1037 tokens, 9 nodes, 16/8 heads 9.7 us, in a cluster of 8 (of these 5 are the chain of
 // loads, a tile's S, softmax and P V, and 3 the two meetings and the join); 13 of 203 .. 3001, 5 .. 33 nodes, 32/8 31.9 us
 // (2.8 TB/s: 6 us until the first tiles are there, 7 the join); 4 of 24000 .. 40960, 33 .. 64 nodes, 8/2 45.8 us (2.9 TB/s, 560 TFLOP/s);
-// 128 of 512 .. 4096, 64 nodes, 32/8 324 us (4.1 TB/s, 950 TFLOP/s; 340 where the power cap sets in, up to 400 with L2 flushed between
-// calls): the softmax chain of a tile, about 3100 cycles for both halves against 2048 of tensor work.
+// 128 of 512 .. 4096, 64 nodes, 32/8 336 to 349 us (3.8 to 4.0 TB/s, 890 to 920 TFLOP/s) in bursts of 20 calls between rests, at 1965 MHz, and 405 to 412 on end, at the power
+// cap and 1390 to 1460 MHz, eagerly as in graphs: the softmax chain of a tile, about 3100 cycles for both halves against 2048 of tensor work.
 #include <atomic>
 #include <climits>
 #include <cmath>
@@ -48,9 +49,9 @@ constexpr int kTrThreads = 512;
 constexpr int kTrRingK = 2, kTrRingV = 3;     // tiles of K and V in shared memory
 constexpr int kTrItems = 4;                   // items in flight
 constexpr float kTrRescale = 8.0f;
-// The line's measure: cost of a key tile and of a unit by itself, with at most QT nodes (a step per tile) and with more (two).  Fitted to
-// the cycles of a CTA's P V thread: 256 chains of 4 nodes, bound by memory, 2210 a tile and 2380 a unit; 13 ragged trees about
-// 1300 and 3300 a tile of either kind; 128 trees of 64 nodes 3090 a tile and 11300 a unit.
+// The line's measure: cost of a key tile and of a unit by itself, with at most QT nodes (a step per tile) and with more (two).  Between
+// the cycles that a CTA's P V thread took: 256 chains of 4 nodes, bound by memory, 2210 a tile and 2380 a unit (their steps no longer come here by themselves,
+// but among larger trees); 13 ragged trees about 1300 and 3300 a tile of either kind; 128 trees of 64 nodes 3090 a tile and 11300 a unit.
 struct TcLine {
   static constexpr int kKeys = kTrKv;
   static constexpr int kTileSplit = 4, kUnitSplit = 5, kTilePair = 7, kUnitPair = 24;
@@ -69,12 +70,6 @@ struct TreeItem {
   int turn;             // the half that takes the unit's first step
   int partial;          // -1: the whole unit, else where its partial results go
 };
-
-// 1-D bulk copy global -> shared, completion counted on an mbarrier (addresses and size multiples of 16).
-__device__ __forceinline__ void tree_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
 
 // A key tile of K or V into its place: in one box per half of the dims; of a sequence's last tile only what it has (`left` keys), in
 // boxes of 16 rows.

@@ -186,11 +186,19 @@ __device__ __forceinline__ void tree_share(const TreeParams& p, int block_nodes,
   }
 }
 
-// Cost of a tile and of a unit in the line of tree_small.cu.
+// Cost of a tile and of a unit in the line of tree_small.cu: a unit, with its rows, its last accumulators and its part in the join, weighs as much as 4.5
+// tiles.  Us with 0 | 2.25 | 4.5 | 9, calls on end in a graph: 256 chains of 4 nodes on 100 .. 2048 tokens at 16/8 heads 221 | 198 | 190 | 190, 64 of 2 .. 10 on
+// 500 .. 3000 at 4/2 40.1 | 36.4 | 34.4 | 33.8, 256 of 3 .. 9 on 100 .. 1000 at 8/4 94.5 | 81.0 | 81.1 | 81.7, 64 of 3 on 500 .. 3000 at 4/2 31.0 | 30.7 | 29.8 | 30.5.
 struct SmLine {
   static constexpr int kKeys = 64;
   static constexpr int kTileSplit = 4, kUnitSplit = 18, kTilePair = 4, kUnitPair = 18;
 };
+// 1-D bulk copy global -> shared, completion counted on an mbarrier (addresses and size multiples of 16).
+__device__ __forceinline__ void tree_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+
 // Few nodes (tree_small.cu): up to 16 rows to a unit, G <= 16; K/V maps with boxes of 64 and of 16 tokens.
 int launch_tree_small(const TreeParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, const CUtensorMap& map_k16,
                       const CUtensorMap& map_v16, int ctas, cudaStream_t stream);

@@ -10,7 +10,7 @@
 // a unit a group leaves its accumulators in the stage of its last tile, which goes back to the ring when the epilogue warps have
 // joined them: the consumers go on with the next unit meanwhile, and the room costs nothing.
 //
-// 256 chains of 4 nodes on 100 .. 2048 tokens at 16/8 heads: 182 to 189 us with the join, 6.0 to 6.2 TB/s (a copy: 6.55); 1 node 179.
+// 256 chains of 4 nodes on 100 .. 2048 tokens at 16/8 heads: 188 us with the launch for large trees and the join, 6.0 TB/s (a copy: 6.55); 1 node 180.
 #include <atomic>
 
 #include "../../include/b200_attn.h"
@@ -36,11 +36,6 @@ struct SmallItem {
   int count;            // tiles of the CTA in front of it
   int partial;          // -1: the whole unit, else where its partial results go
 };
-
-__device__ __forceinline__ void small_bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
-}
 
 // A consumer warp's running state: rows lane / 4 and lane / 4 + 8.
 struct SmallAcc {
@@ -251,7 +246,7 @@ tree_small_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_k,
           for (int x = 0, r = 0; x < nodes; ++x) {
             const __nv_bfloat16* const from = p.q + static_cast<long long>(q_row + x) * p.q_row_stride + h * G * 128;
 #pragma unroll 1
-            for (int g = 0; g < G; ++g, ++r) small_bulk_load(sQ + b * kSmQ + r * kSmQRow, from + g * 128, 256, &bar_q_full[b]);
+            for (int g = 0; g < G; ++g, ++r) tree_bulk_load(sQ + b * kSmQ + r * kSmQRow, from + g * 128, 256, &bar_q_full[b]);
           }
         }
       }
